@@ -12,6 +12,7 @@ import functools
 import math
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -1952,3 +1953,146 @@ def gru_scan(y, src, col_z: int, col_u: int, col_g: int, z_b, u_b, state,
     else:
         torch_ref.gru_scan(y, src, col_z, col_u, col_g, z_b, u_b, state,
                            seq_first, seq_rows, state_slots, pos32)
+
+
+# --- rows in 8 bits, their products, adapters beside a projection ----------
+# ops/csrc/fp8_rows.hip, fp8_gemm.hip and lora.hip in `_hip_fp8.so`.
+
+_FP8 = None
+
+
+def _load_fp8():
+    """Load `_hip_fp8.so` (rows in 8 bits, their products, adapters), compiling
+    it in-tree first when no built library is there."""
+    global _FP8
+    if _FP8 is not None:
+        return _FP8
+    import importlib.util
+
+    from .build import FP8_SO_PATH, build_fp8
+
+    if not FP8_SO_PATH.exists():
+        build_fp8()
+    spec = importlib.util.spec_from_file_location(
+        "gpustack_amd.ops._hip_fp8", FP8_SO_PATH)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    _FP8 = mod
+    return mod
+
+
+def _fp8_backend(t: torch.Tensor):
+    return _load_fp8() if t.is_cuda else None
+
+
+class Rows8(NamedTuple):
+    """Rows in 8 bits: row t is q[t] * scale[t]. `rows`: the same rows in the
+    type that they were rounded from, where the caller asked for them."""
+
+    q: torch.Tensor                    # e4m3 [T, H]
+    scale: torch.Tensor                # fp32 [T]
+    rows: torch.Tensor | None = None   # [T, H]
+
+
+def _rows8(x, width: int) -> Rows8:
+    return Rows8(torch.empty(x.shape[0], width, dtype=torch.float8_e4m3fn,
+                             device=x.device),
+                 torch.empty(x.shape[0], dtype=torch.float32, device=x.device))
+
+
+def rows_fp8(x) -> Rows8:
+    """x [T, H] in 8 bits (torch_ref.fp8_rows has the semantics). On the GPU
+    bf16, rows of any stride that keeps them at multiples of 16 bytes."""
+    k = _fp8_backend(x)
+    if k is None:
+        return Rows8(*torch_ref.fp8_rows(x))
+    r = _rows8(x, x.shape[1])
+    k.fp8_rows(0, r.q, r.scale, None, None, x, None, None, 0.0)
+    return r
+
+
+def silu_and_mul_fp8(x) -> Rows8:
+    """silu(gate) * up of x = [gate | up] in 8 bits, rounded once."""
+    k = _fp8_backend(x)
+    if k is None:
+        return Rows8(*torch_ref.silu_and_mul_fp8(x))
+    r = _rows8(x, x.shape[1] // 2)
+    k.fp8_rows(1, r.q, r.scale, None, None, x, None, None, 0.0)
+    return r
+
+
+def add_rms_norm_fp8(x, residual, weight, eps: float, rows: bool = False):
+    """(the RMS norm of x + residual in 8 bits, x + residual): the sum is held
+    in x's type, the norm of it rounded once. Without a residual the sum is x
+    itself. `rows`: the norm in x's type too, for adapters (lora_add) beside
+    the 8-bit product."""
+    k = _fp8_backend(x)
+    if k is None:
+        q, scale, h, total = torch_ref.add_rms_norm_fp8(x, residual, weight, eps)
+        return Rows8(q, scale, h if rows else None), total
+    r = _rows8(x, x.shape[1])
+    like = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = like() if residual is not None else None
+    h = like() if rows else None
+    k.fp8_rows(2, r.q, r.scale, total, h, x, residual, weight, eps)
+    return Rows8(r.q, r.scale, h), x if total is None else total
+
+
+def _fp8_plan(M: int, N: int, K: int):
+    """(rows, columns of a tile in 16, parts over k) of an 8-bit product."""
+    mt = 2 if M <= 32 else 4 if M <= 64 else 8
+    nt = 8
+    tiles = -(-M // (16 * mt)) * -(-N // (16 * nt))
+    return mt, nt, max(1, min(512 // tiles, -(-K // 1024)))
+
+
+def linear_fp8(q, scale, w, w_scale, bias=None, dtype=torch.bfloat16):
+    """q w^T of e4m3 rows and weights times a scale a row and a scale a column,
+    plus bias, rounded once (torch_ref.linear_fp8). K is a multiple of 16, N of
+    8. `dtype`: of the result; on the GPU bf16."""
+    k = _fp8_backend(q)
+    if k is None:
+        return torch_ref.linear_fp8(q, scale, w, w_scale, bias, dtype)
+    M, N = q.shape[0], w.shape[0]
+    out = torch.empty(M, N, dtype=dtype, device=q.device)
+    if M <= 16:
+        k.fp8_rows_gemm(out, q, scale, w, w_scale, bias, 16)
+    else:
+        k.fp8_tile(out, q, scale, w, w_scale, bias, *_fp8_plan(M, N, q.shape[1]))
+    return out
+
+
+def build_lora_rows(slots, n_slots: int, device):
+    """What lora_add reads of a batch: `slots` has each row's adapter, below 0
+    or from n_slots on none. Returns (order, starts), int32: the rows of slot s
+    are order[starts[s]:starts[s + 1]], rows without an adapter behind all of
+    them."""
+    order, starts = lora_rows(slots, n_slots)
+    return tuple(to_device([(order, torch.int32), (starts, torch.int32)], device))
+
+
+def lora_rows(slots, n_slots: int):
+    """build_lora_rows' lists as host arrays."""
+    import numpy as np
+
+    key = np.asarray(slots, dtype=np.int64)
+    key = np.where((key < 0) | (key >= n_slots), n_slots, key)
+    order = np.argsort(key, kind="stable").astype(np.int32)
+    starts = np.searchsorted(key[order], np.arange(n_slots + 1)).astype(np.int32)
+    return order, starts
+
+
+def lora_add(out, x, a, b, order, starts, ranks, ends) -> None:
+    """out[t] += the low-rank product x[t] a[s]^T b[s]^T of row t's adapter s, in
+    place: a [S, P R, K], b [S, N, R], ranks int32 [S], of which the first
+    `ranks[s]` of R are used and nothing behind them is; `ends`: where the P
+    parts of the projection (q, k, v; gate, up) end in its N columns, part p
+    reading the middle values p R .. of a. order, starts: build_lora_rows; a row
+    is named once at most, and rows that no slot names are left as they are. On
+    the GPU bf16 with fp32 sums, rows of out and x at multiples of 16 bytes, R
+    up to 256; K, R and the ends are multiples of 8."""
+    k = _fp8_backend(x)
+    if k is not None:
+        k.lora_add(out, x, a, b, order, starts, ranks, list(ends))
+    else:
+        torch_ref.lora_add(out, x, a, b, order, starts, ranks, ends)

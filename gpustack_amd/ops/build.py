@@ -49,6 +49,10 @@ STREAMS_SO_PATH = PKG_DIR / "_hip_streams.so"
 STREAMS_SOURCES = ["hyperrows32.hip", "gru_scan.hip", "short_conv.hip",
                    "stream_bindings.cpp"]
 
+# rows in 8 bits, their products, adapters beside a projection
+FP8_SO_PATH = PKG_DIR / "_hip_fp8.so"
+FP8_SOURCES = ["fp8_rows.hip", "fp8_gemm.hip", "lora.hip", "fp8_bindings.cpp"]
+
 
 def _torch_paths():
     import torch
@@ -179,6 +183,12 @@ def build_streams(verbose: bool = False, force: bool = True) -> Path:
                         verbose, force)
 
 
+def build_fp8(verbose: bool = False, force: bool = True) -> Path:
+    """Compile rows in 8 bits, their products and the adapters beside a
+    projection into `_hip_fp8.so`."""
+    return _build_small("_hip_fp8", FP8_SOURCES, FP8_SO_PATH, verbose, force)
+
+
 def _build_small(ext_name: str, sources: list[str], so_path: Path,
                  verbose: bool, force: bool) -> Path:
     """Compile one small extension, its files in parallel. Objects are
@@ -233,11 +243,15 @@ if __name__ == "__main__":
     elif "--streams" in sys.argv:
         build_streams(verbose=True)
         print(f"built {STREAMS_SO_PATH}")
+    elif "--fp8" in sys.argv:
+        build_fp8(verbose=True)
+        print(f"built {FP8_SO_PATH}")
     else:
         build(verbose=True, force="--force" in sys.argv)
         build_latent(verbose=True)
         build_paged(verbose=True)
         build_state(verbose=True)
         build_streams(verbose=True)
+        build_fp8(verbose=True)
         print(f"built {SO_PATH} {LATENT_SO_PATH} {PAGED_SO_PATH} "
-              f"{STATE_SO_PATH} {STREAMS_SO_PATH}")
+              f"{STATE_SO_PATH} {STREAMS_SO_PATH} {FP8_SO_PATH}")

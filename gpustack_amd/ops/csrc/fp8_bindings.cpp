@@ -1,0 +1,204 @@
+// Torch bindings for rows in 8 bits (fp8_rows.hip), their products (fp8_gemm.hip) and
+// the adapters beside a projection (lora.hip). Every shape, stride and address that a
+// kernel or its grid assumes is checked here on the host before the launch; VALUES
+// inside index tensors are bounded in the kernels.
+#include <torch/extension.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+
+int fp8_rows_most();
+void fp8_rows_launch(int, void*, float*, void*, void*, const void*, long, const void*, const void*, float, int, int, hipStream_t);
+void fp8_rows_gemm_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, hipStream_t);
+bool fp8_tile_has(int, int);
+void fp8_tile_launch(void*, void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, int, hipStream_t);
+int lora_most_rank();
+void lora_launch(void*, long, float*, const void*, long, const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, const int*, int, int, int, hipStream_t);
+
+#define HIP_CHECK_LAST()                                                     \
+  do {                                                                       \
+    hipError_t e_ = hipGetLastError();                                       \
+    TORCH_CHECK(e_ == hipSuccess, "HIP kernel launch failed: ",              \
+                hipGetErrorString(e_));                                      \
+  } while (0)
+
+namespace {
+
+using at::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+hipStream_t cur_stream(const Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// a dense operand on the device of `like`, at an address the kernels' 16-byte accesses take
+void chk(const Tensor& t, const char* name, at::ScalarType ty, const Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be on the GPU of the other operands");
+  TORCH_CHECK(t.scalar_type() == ty, name, " must be ", ty, ", not ", t.scalar_type());
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(t.numel() == 0 || (unsigned long)t.data_ptr() % 16 == 0, name,
+              " must begin at a multiple of 16 bytes");
+}
+
+// bf16 rows of any row stride that keeps them at multiples of 16 bytes: the stride
+long chk_rows(const Tensor& t, const char* name, const Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be on the GPU of the other operands");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bf16");
+  TORCH_CHECK(t.dim() == 2 && (t.size(1) == 1 || t.stride(1) == 1), name,
+              " must be rows of neighbouring elements");
+  const long stride = t.size(0) > 1 ? t.stride(0) : (t.size(1) + 7) / 8 * 8;
+  TORCH_CHECK(t.numel() == 0 || ((unsigned long)t.data_ptr() % 16 == 0 &&
+                                 stride % 8 == 0 && stride >= t.size(1)), name,
+              " must have its rows at multiples of 16 bytes, none over another");
+  return stride;
+}
+
+void fp8_rows(int64_t source, Tensor q, Tensor scale, OptTensor sum, OptTensor rows,
+              Tensor x, OptTensor residual, OptTensor weight, double eps) {
+  TORCH_CHECK(source >= 0 && source <= 2, "fp8_rows: no such source");
+  const long xs = chk_rows(x, "x", x);
+  const long T = x.size(0), W = x.size(1), H = source == 1 ? W / 2 : W;
+  TORCH_CHECK(T < 1l << 31 && H >= 8 && H % 8 == 0 && H <= fp8_rows_most() &&
+              (source != 1 || W % 2 == 0),
+              "fp8_rows: rows of ", W, " elements: the result's are a multiple of 8, at most ",
+              fp8_rows_most());
+  chk(q, "q", at::kFloat8_e4m3fn, x);
+  chk(scale, "scale", at::kFloat, x);
+  TORCH_CHECK(q.dim() == 2 && q.size(0) == T && q.size(1) == H && scale.dim() == 1 &&
+              scale.size(0) == T, "fp8_rows: shapes of the result");
+  TORCH_CHECK(residual.has_value() == sum.has_value(), "fp8_rows: residual and its sum");
+  TORCH_CHECK(weight.has_value() == (source == 2) && (source == 2 || !(residual || rows)),
+              "fp8_rows: what belongs to the norm");
+  if (weight) {
+    chk(*weight, "weight", at::kBFloat16, x);
+    TORCH_CHECK(weight->dim() == 1 && weight->size(0) == H, "fp8_rows: weight's size");
+  }
+  for (const auto& t : {std::make_pair(&residual, "residual"), std::make_pair(&sum, "sum"),
+                        std::make_pair(&rows, "rows")})
+    if (t.first->has_value()) {
+      chk(**t.first, t.second, at::kBFloat16, x);
+      TORCH_CHECK((*t.first)->dim() == 2 && (*t.first)->size(0) == T &&
+                  (*t.first)->size(1) == H, "fp8_rows: shape of ", t.second);
+    }
+  if (T == 0) return;
+  const at::DeviceGuard guard(x.device());
+  auto at = [](const OptTensor& t) { return t ? t->data_ptr() : nullptr; };
+  fp8_rows_launch((int)source, q.data_ptr(), scale.data_ptr<float>(), at(sum), at(rows),
+                  x.data_ptr(), xs, at(residual), at(weight), (float)eps, (int)T, (int)H,
+                  cur_stream(x));
+  HIP_CHECK_LAST();
+}
+
+struct Product { int M, N, K; const void* bias; };
+
+Product chk_product(const Tensor& out, const Tensor& x, const Tensor& xs, const Tensor& w,
+                    const Tensor& ws, const OptTensor& bias) {
+  chk(x, "x", at::kFloat8_e4m3fn, x);
+  chk(xs, "x_scale", at::kFloat, x);
+  chk(w, "w", at::kFloat8_e4m3fn, x);
+  chk(ws, "w_scale", at::kFloat, x);
+  chk(out, "out", at::kBFloat16, x);
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1),
+              "fp8 product: x [M, K] and w [N, K]");
+  const long M = x.size(0), K = x.size(1), N = w.size(0);
+  TORCH_CHECK(K >= 16 && K % 16 == 0 && N >= 8 && N % 8 == 0 && K < 1l << 31 &&
+              N < 1l << 31 && M < 1l << 31,
+              "fp8 product: K a multiple of 16 and N one of 8, not ", K, " and ", N);
+  TORCH_CHECK(xs.dim() == 1 && xs.size(0) == M && ws.dim() == 1 && ws.size(0) == N,
+              "fp8 product: a scale a row and a scale a column");
+  TORCH_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == N,
+              "fp8 product: out [M, N]");
+  if (bias) {
+    chk(*bias, "bias", at::kBFloat16, x);
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "fp8 product: bias's size");
+  }
+  return {(int)M, (int)N, (int)K, bias ? bias->data_ptr() : nullptr};
+}
+
+void fp8_rows_gemm(Tensor out, Tensor x, Tensor xs, Tensor w, Tensor ws, OptTensor bias,
+                   int64_t cols) {
+  const Product p = chk_product(out, x, xs, w, ws, bias);
+  TORCH_CHECK(p.M <= 16 && (cols == 16 || cols == 32), "fp8_rows_gemm: plan");
+  if (p.M == 0) return;
+  const at::DeviceGuard guard(x.device());
+  fp8_rows_gemm_launch(out.data_ptr(), x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(),
+                       ws.data_ptr<float>(), p.bias, p.M, p.N, p.K, (int)cols,
+                       cur_stream(x));
+  HIP_CHECK_LAST();
+}
+
+void fp8_tile(Tensor out, Tensor x, Tensor xs, Tensor w, Tensor ws, OptTensor bias,
+              int64_t mt, int64_t nt, int64_t splits) {
+  const Product p = chk_product(out, x, xs, w, ws, bias);
+  TORCH_CHECK(fp8_tile_has(mt, nt) && splits >= 1 && splits <= (p.K + 127) / 128 &&
+              (p.N + 16 * nt - 1) / (16 * nt) * splits < 1l << 31 &&
+              p.M <= 65535l * 16 * mt,
+              "fp8_tile: plan");
+  if (p.M == 0) return;
+  const at::DeviceGuard guard(x.device());
+  Tensor parts;
+  if (splits > 1)
+    parts = at::empty({splits, p.M, p.N}, x.options().dtype(at::kFloat));
+  fp8_tile_launch(out.data_ptr(), splits > 1 ? parts.data_ptr() : nullptr, x.data_ptr(),
+                  xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), p.bias, p.M,
+                  p.N, p.K, (int)mt, (int)nt, (int)splits, cur_stream(x));
+  HIP_CHECK_LAST();
+}
+
+void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor starts,
+              Tensor ranks, std::vector<int64_t> ends) {
+  const long os = chk_rows(out, "out", x), xs = chk_rows(x, "x", x);
+  chk(a, "a", at::kBFloat16, x);
+  chk(b, "b", at::kBFloat16, x);
+  const long rows = x.size(0), K = x.size(1), N = out.size(1), P = ends.size();
+  TORCH_CHECK(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) && a.size(2) == K &&
+              b.size(1) == N && out.size(0) == rows,
+              "lora_add: x [T, K], out [T, N], a [S, P R, K], b [S, N, R]");
+  const long S = a.size(0), R = b.size(2);
+  TORCH_CHECK(P >= 1 && P <= 4 && a.size(1) == P * R && R >= 8 && R % 8 == 0 &&
+              R <= lora_most_rank() && K >= 8 && K % 8 == 0,
+              "lora_add: 1 to 4 parts, ranks a multiple of 8 up to ", lora_most_rank(),
+              ", K a multiple of 8");
+  int e[4] = {0, 0, 0, 0};
+  for (long i = 0; i < P; ++i) {
+    TORCH_CHECK(ends[i] > (i ? ends[i - 1] : 0) && ends[i] % 8 == 0 && ends[i] <= N,
+                "lora_add: parts end at rising multiples of 8, the last at N");
+    e[i] = (int)ends[i];
+  }
+  TORCH_CHECK(ends[P - 1] == N, "lora_add: parts end at rising multiples of 8, the last at N");
+  for (const auto& t : {std::make_pair(&order, "order"), std::make_pair(&starts, "starts"),
+                        std::make_pair(&ranks, "ranks")}) {
+    TORCH_CHECK(t.first->is_cuda() && t.first->device() == x.device() &&
+                t.first->scalar_type() == at::kInt && t.first->is_contiguous() &&
+                t.first->dim() == 1, t.second, " must be int32 on the GPU of the others");
+  }
+  const long T = order.size(0);
+  TORCH_CHECK(starts.size(0) == S + 1 && ranks.size(0) == S,
+              "lora_add: S + 1 starts and S ranks");
+  TORCH_CHECK(T <= rows && rows < 1l << 31 && S < 1l << 24 && N < 1l << 31 && K < 1l << 31 &&
+              (N + 255) / 256 + P <= 65535, "lora_add: sizes");
+  if (T == 0 || S == 0) return;
+  const at::DeviceGuard guard(x.device());
+  // tiles of 64 rows where a slot has half of one on average, else of 16. k is cut until
+  // there are two workgroups a CU, each wave having a unit of 64 k of its own at least
+  const int tt = T >= 32 * std::min(S, T) ? 4 : 1;
+  const long tiles = std::min(T, (T + std::min(S, T) * (16 * tt - 1)) / (16 * tt));
+  const long groups = (P * ((R + 15) / 16) + tt - 1) / tt;
+  const long splits = std::max(1l, std::min({512 / (tiles * groups), (K + 255) / 256, 16l}));
+  Tensor h = at::empty({splits, T, P * R}, x.options().dtype(at::kFloat));
+  lora_launch(out.data_ptr(), os, h.data_ptr<float>(), x.data_ptr(), xs, a.data_ptr(),
+              b.data_ptr(), order.data_ptr<int>(), starts.data_ptr<int>(),
+              ranks.data_ptr<int>(), (int)rows, (int)T, (int)S, (int)N, (int)K, (int)P, e,
+              (int)R, tt, (int)splits, cur_stream(x));
+  HIP_CHECK_LAST();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("fp8_rows", &fp8_rows);
+  m.def("fp8_rows_gemm", &fp8_rows_gemm);
+  m.def("fp8_tile", &fp8_tile);
+  m.def("lora_add", &lora_add);
+}

@@ -1,0 +1,170 @@
+// Rows in 8 bits for MI355X (gfx950): a row v becomes e4m3 values q and one fp32 scale
+// s with v = q s, for the products of fp8_gemm.hip. v comes from
+//   NORM   v = r rsqrt(mean r^2 + eps) w, r = bf16(x + residual) or x
+//   SILU   v = g / (1 + e^-g) u, x = [g | u]
+//   PLAIN  v = x
+// in fp32 and is rounded once, to nearest: q = e4m3(v / s), s = max(|v|) / 448, which
+// makes the largest value the largest that e4m3 has, and at least 2^-100, which gives
+// rows of zeros a scale and every s a reciprocal. A row with an infinity or a NaN has
+// none that could be told from its products: its maximum is taken over the bits, where
+// they are above every number, so its scale is the infinity or NaN and so are its
+// products.
+//
+// Bound by memory: each row is read once and held in registers between its sums, its
+// maximum and its rounding. A row takes a wave up to 1024 channels (four rows a
+// workgroup), 256 threads up to 8192, 1024 beyond.
+#include "common.h"
+
+namespace {
+
+enum RowSource { PLAIN, SILU, NORM };
+
+constexpr float TOP = 448.f, LEAST = 0x1p-100f;
+
+DEVICE_INLINE unsigned wave_max_bits(unsigned v) {
+  auto f = [](unsigned u) { return __builtin_bit_cast(float, u); };
+  auto u = [](float x) { return __builtin_bit_cast(unsigned, x); };
+  f32x2 p = with_lane<32>(f(v));
+  p = with_lane<16>(f(max(u(p[0]), u(p[1]))));
+  v = max(u(p[0]), u(p[1]));
+  v = max(v, u(row_turned<8>(f(v))));
+  v = max(v, u(row_turned<4>(f(v))));
+  v = max(v, u(row_turned<2>(f(v))));
+  return max(v, u(row_turned<1>(f(v))));
+}
+
+// G threads a row, NV times 8 values each; 256 / G rows a workgroup below 256.
+template <int SRC, int G, int NV>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
+    unsigned char* __restrict__ q, float* __restrict__ scale,
+    unsigned short* __restrict__ sum,        // NORM: x + residual, with a residual
+    unsigned short* __restrict__ rows,       // NORM: v in bf16, or null
+    const unsigned short* __restrict__ x, long xs,
+    const unsigned short* __restrict__ residual,
+    const unsigned short* __restrict__ weight, float eps, int T, int H) {
+  constexpr int ROWS = G < 256 ? 256 / G : 1, WAVES = G / WAVE_SIZE;
+  __shared__ float part[2][WAVES];
+  const int t = threadIdx.x % G;
+  const long row = (long)blockIdx.x * ROWS + threadIdx.x / G;
+  if (G < 256 && row >= T) return;           // whole waves; none waits for another
+  const unsigned short* xr = x + row * xs;
+
+  float v[NV][8];
+  float squares = 0.f;
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + t) * 8;
+    if (c < H) {
+      const u16x8 a = *reinterpret_cast<const u16x8*>(xr + c);
+      if constexpr (SRC == SILU) {
+        const u16x8 b = *reinterpret_cast<const u16x8*>(xr + H + c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v[i][j] = over_one_plus_exp(bf2f(a[j]), bf2f(a[j])) * bf2f(b[j]);
+      } else {
+        u16x8 r = a;
+        if (SRC == NORM && residual) {
+          const u16x8 b = *reinterpret_cast<const u16x8*>(residual + row * H + c);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) r[j] = f2bf(bf2f(a[j]) + bf2f(b[j]));
+          *reinterpret_cast<u16x8*>(sum + row * H + c) = r;
+        }
+        bf8_to_f32(r, v[i]);
+        if constexpr (SRC == NORM)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) squares += v[i][j] * v[i][j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+  }
+  if constexpr (SRC == NORM) {
+    squares = wave_reduce_sum(squares);
+    if constexpr (WAVES > 1) {
+      if (t % WAVE_SIZE == 0) part[0][t / WAVE_SIZE] = squares;
+      __syncthreads();
+      squares = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) squares += part[0][w];
+    }
+    const float inv = 1.f / sqrtf(squares / (float)H + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + t) * 8;
+      if (c < H) {
+        const u16x8 w = *reinterpret_cast<const u16x8*>(weight + c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * bf2f(w[j]);
+        if (rows) *reinterpret_cast<u16x8*>(rows + row * H + c) = f32_to_bf8(v[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      top = max(top, __builtin_bit_cast(unsigned, v[i][j]) & 0x7fffffffu);
+  top = wave_max_bits(top);
+  if constexpr (WAVES > 1) {
+    if (t % WAVE_SIZE == 0) part[1][t / WAVE_SIZE] = __builtin_bit_cast(float, top);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      top = max(top, __builtin_bit_cast(unsigned, part[1][w]));
+  }
+  const float most = __builtin_bit_cast(float, top);
+  // a NaN is neither below nor above the least scale, and stays
+  const float s = most / TOP < LEAST ? LEAST : most / TOP;
+  const float turn = 1.f / s;
+  if (t == 0) scale[row] = s;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + t) * 8;
+    if (c < H) {
+      uint2 o;
+      int lo = 0, hi = 0;
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][0] * turn, v[i][1] * turn, lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][2] * turn, v[i][3] * turn, lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][4] * turn, v[i][5] * turn, hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][6] * turn, v[i][7] * turn, hi, true);
+      o.x = lo;
+      o.y = hi;
+      *reinterpret_cast<uint2*>(q + row * H + c) = o;
+    }
+  }
+}
+
+}  // namespace
+
+int fp8_rows_most() { return 65536; }
+
+// source: RowSource. H: channels of a result row, a multiple of 8.
+void fp8_rows_launch(int source, void* q, float* scale, void* sum, void* rows,
+                     const void* x, long xs, const void* residual, const void* weight,
+                     float eps, int T, int H, hipStream_t s) {
+  auto go = [&](auto kernel, int g) {
+    const int each = g < 256 ? 256 / g : 1;
+    hipLaunchKernelGGL(kernel, dim3((T + each - 1) / each), dim3(g < 256 ? 256 : g), 0, s,
+                       (unsigned char*)q, scale, (unsigned short*)sum,
+                       (unsigned short*)rows, (const unsigned short*)x, xs,
+                       (const unsigned short*)residual, (const unsigned short*)weight,
+                       eps, T, H);
+  };
+  auto by_size = [&](auto src) {
+    constexpr int SRC = decltype(src)::value;
+    if (H <= 512) go(fp8_rows_kernel<SRC, 64, 1>, 64);
+    else if (H <= 1024) go(fp8_rows_kernel<SRC, 64, 2>, 64);
+    else if (H <= 2048) go(fp8_rows_kernel<SRC, 256, 1>, 256);
+    else if (H <= 4096) go(fp8_rows_kernel<SRC, 256, 2>, 256);
+    else if (H <= 6144) go(fp8_rows_kernel<SRC, 256, 3>, 256);
+    else if (H <= 8192) go(fp8_rows_kernel<SRC, 256, 4>, 256);
+    else if (H <= 16384) go(fp8_rows_kernel<SRC, 1024, 2>, 1024);
+    else if (H <= 32768) go(fp8_rows_kernel<SRC, 1024, 4>, 1024);
+    else go(fp8_rows_kernel<SRC, 1024, 8>, 1024);
+  };
+  if (source == SILU) by_size(std::integral_constant<int, SILU>{});
+  else if (source == NORM) by_size(std::integral_constant<int, NORM>{});
+  else by_size(std::integral_constant<int, PLAIN>{});
+}

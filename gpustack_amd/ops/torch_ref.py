@@ -1128,3 +1128,94 @@ def gru_scan(y: torch.Tensor, src: torch.Tensor, col_z: int, col_u: int,
             S = (1.0 - z[t]) * S + z[t] * c[t]
             y[t] = (S * g[t]).to(y.dtype)
         st[slot] = S
+
+
+# --- rows in 8 bits, their products, adapters beside a projection ----------
+
+FP8_TOP = 448.0            # the largest e4m3 value
+FP8_LEAST = 2.0 ** -100    # the least scale
+
+
+def _want(ok: bool, what: str) -> None:
+    if not ok:
+        raise RuntimeError(what)
+
+
+def fp8_rows(v: torch.Tensor):
+    """v [T, H] -> (e4m3 [T, H], fp32 [T]): v / scale rounded to nearest, the
+    scale a row's largest absolute value / 448, at least 2^-100. A row with an
+    infinity or a NaN has that for its scale."""
+    _want(v.dim() == 2 and v.shape[1] >= 8 and v.shape[1] % 8 == 0
+          and v.shape[1] <= 65536,
+          "fp8_rows: rows of a multiple of 8 elements, at most 65536")
+    v = v.float()
+    scale = (v.abs().amax(1) / FP8_TOP).clamp(min=FP8_LEAST)
+    return (v / scale[:, None]).to(torch.float8_e4m3fn), scale
+
+
+def silu_and_mul_fp8(x: torch.Tensor):
+    _want(x.dim() == 2 and x.shape[1] % 2 == 0, "fp8_rows: [gate | up] rows")
+    g, u = x.float().chunk(2, 1)
+    return fp8_rows(g / (1 + torch.exp(-g)) * u)
+
+
+def add_rms_norm_fp8(x, residual, weight, eps: float):
+    """(e4m3 rows, scales, the rows in x's type, x + residual in x's type)."""
+    _want(weight.dim() == 1 and x.dim() == 2 and weight.shape[0] == x.shape[1],
+          "fp8_rows: weight's size")
+    total = x
+    if residual is not None:
+        _want(residual.shape == x.shape, "fp8_rows: shape of residual")
+        total = (x.float() + residual.float()).to(x.dtype)
+    t = total.float()
+    v = t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps) * weight.float()
+    q, scale = fp8_rows(v)
+    return q, scale, v.to(x.dtype), total
+
+
+def linear_fp8(q, scale, w, w_scale, bias=None, dtype=torch.bfloat16):
+    _want(q.dim() == 2 and w.dim() == 2 and q.shape[1] == w.shape[1],
+          "fp8 product: x [M, K] and w [N, K]")
+    M, K = q.shape
+    N = w.shape[0]
+    _want(q.dtype == w.dtype == torch.float8_e4m3fn, "fp8 product: e4m3 operands")
+    _want(K >= 16 and K % 16 == 0 and N >= 8 and N % 8 == 0,
+          f"fp8 product: K a multiple of 16 and N one of 8, not {K} and {N}")
+    _want(scale.shape == (M,) and w_scale.shape == (N,),
+          "fp8 product: a scale a row and a scale a column")
+    _want(bias is None or bias.shape == (N,), "fp8 product: bias's size")
+    y = (q.float() @ w.float().T) * (scale[:, None] * w_scale)
+    return (y if bias is None else y + bias.float()).to(dtype)
+
+
+def lora_add(out, x, a, b, order, starts, ranks, ends) -> None:
+    _want(x.dim() == 2 and out.dim() == 2 and a.dim() == 3 and b.dim() == 3
+          and a.shape[0] == b.shape[0] and a.shape[2] == x.shape[1]
+          and b.shape[1] == out.shape[1] and out.shape[0] == x.shape[0],
+          "lora_add: x [T, K], out [T, N], a [S, P R, K], b [S, N, R]")
+    S, N, R = b.shape
+    P, T = len(ends), x.shape[0]
+    _want(1 <= P <= 4 and a.shape[1] == P * R and R >= 8 and R % 8 == 0
+          and R <= 256 and x.shape[1] % 8 == 0,
+          "lora_add: 1 to 4 parts, ranks a multiple of 8 up to 256, K a "
+          "multiple of 8")
+    _want(all(e > s and e % 8 == 0 for s, e in zip((0, *ends), ends))
+          and ends[-1] == N,
+          "lora_add: parts end at rising multiples of 8, the last at N")
+    _want(starts.shape == (S + 1,) and ranks.shape == (S,),
+          "lora_add: S + 1 starts and S ranks")
+    _want(order.dim() == 1 and order.shape[0] <= T, "lora_add: sizes")
+    starts = starts.tolist()
+    for slot, rank in enumerate(ranks.tolist()):
+        rank = min(max(rank, 0), R)
+        rows = order[max(starts[slot], 0):max(starts[slot + 1], 0)].long()
+        if not rank or not len(rows):
+            continue
+        rows = rows[(rows >= 0) & (rows < T)]
+        xs, first = x[rows].float(), 0
+        delta = []
+        for p, end in enumerate(ends):
+            h = xs @ a[slot, p * R:p * R + rank].float().T
+            delta.append(h @ b[slot, first:end, :rank].float().T)
+            first = end
+        out[rows] = (out[rows].float() + torch.cat(delta, 1)).to(out.dtype)

@@ -1,0 +1,157 @@
+"""Rows in 8 bits, their products and adapters beside a projection: the plain
+forms, their refusals, the batch's lists. The kernels: test_fp8_lora_gpu.py."""
+import numpy as np
+import pytest
+import torch
+
+from gpustack_amd import ops
+
+E4M3 = torch.float8_e4m3fn
+
+
+def _gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def test_rows_are_within_half_a_step():
+    v = torch.randn(5, 64, generator=_gen()).bfloat16()
+    r = ops.rows_fp8(v)
+    assert r.q.dtype == E4M3 and r.rows is None
+    back = r.q.double() * r.scale.double()[:, None]
+    # half a step of e4m3: 2^-4 of a normal value, 2^-10 of the scale below 2^-6
+    # of it; the scale and the quotient are fp32
+    half = torch.maximum(v.double().abs() * 2 ** -4, r.scale.double()[:, None] * 2 ** -10)
+    assert ((back - v.double()).abs() <= half * (1 + 2 ** -20)).all()
+    assert (r.q.float().abs().amax(1) == 448).all()
+
+
+def test_rows_of_zeros_and_without_numbers():
+    v = torch.zeros(4, 16, dtype=torch.bfloat16)
+    v[1, 3] = float("inf")
+    v[2, 5] = float("nan")
+    v[3, 0] = 2.0 ** -120
+    q, scale, _ = ops.rows_fp8(v)
+    assert scale[0] == 2.0 ** -100 and (q[0].float() == 0).all()
+    assert torch.isinf(scale[1]) and torch.isnan(q[1].float()[3])
+    assert torch.isnan(scale[2])
+    assert scale[3] == 2.0 ** -100 and q[3].float()[0] == 0
+
+
+@pytest.mark.parametrize("rows", [False, True])
+def test_norm_is_the_unfused_one(rows):
+    g = _gen(1)
+    x, res = (torch.randn(3, 48, generator=g).bfloat16() for _ in range(2))
+    w = torch.randn(48, generator=g).bfloat16()
+    r, total = ops.add_rms_norm_fp8(x, res, w, 1e-5, rows=rows)
+    assert torch.equal(total, (x.float() + res.float()).bfloat16())
+    h = total.clone()
+    ops.rms_norm(h, total, w, 1e-5)
+    assert (r.rows is not None) == rows and (not rows or torch.equal(r.rows, h))
+    # of the unrounded rows, so a step of e4m3 from those of the rounded ones
+    want = ops.rows_fp8(h)
+    assert torch.allclose(r.scale, want.scale, rtol=2 ** -8)
+    alone, same = ops.add_rms_norm_fp8(total, None, w, 1e-5)
+    assert same is total and torch.equal(alone.q.float(), r.q.float())
+
+
+def test_batch_lists():
+    order, starts = ops.build_lora_rows([2, -1, 0, 2, 7, 0], 3, "cpu")
+    assert order.dtype == starts.dtype == torch.int32
+    assert order.tolist() == [2, 5, 0, 3, 1, 4] and starts.tolist() == [0, 2, 2, 4]
+    order, starts = ops.build_lora_rows([], 2, "cpu")
+    assert order.numel() == 0 and starts.tolist() == [0, 0, 0]
+
+
+def lora_case(T, K, ends, S, R, slots, ranks, seed, dtype=torch.bfloat16):
+    g = _gen(seed)
+    N = ends[-1]
+    out = torch.randn(T, N, generator=g).to(dtype)
+    x = torch.randn(T, K, generator=g).to(dtype)
+    a = (torch.randn(S, len(ends) * R, K, generator=g) * K ** -.5).to(dtype)
+    b = (torch.randn(S, N, R, generator=g) * R ** -.5).to(dtype)
+    return out, x, a, b, torch.tensor(slots), torch.tensor(ranks, dtype=torch.int32)
+
+
+def lora_exact(out, x, a, b, slots, ranks, ends):
+    """In 64 bits, row by row; with it the sum of every term's size, which the
+    roundings of h are relative to."""
+    want, size = out.double(), torch.zeros(out.shape, dtype=torch.float64)
+    R = b.shape[2]
+    for t, s in enumerate(slots.tolist()):
+        if not 0 <= s < len(ranks):
+            continue
+        r, first = int(ranks[s]), 0
+        for p, end in enumerate(ends):
+            down, up = a[s, p * R:p * R + r].double(), b[s, first:end, :r].double()
+            h = down @ x[t].double()
+            want[t, first:end] += up @ h
+            size[t, first:end] = up.abs() @ (down.abs() @ x[t].double().abs())
+            first = end
+    return want, size
+
+
+def test_lora_plain_form():
+    ends = (16, 24, 40)
+    slots = [1, -1, 0, 2, 2, 1, 9]
+    out, x, a, b, s, ranks = lora_case(7, 32, ends, 3, 8, slots, [8, 3, 0], 3)
+    for i, r in enumerate(ranks.tolist()):       # nothing behind the rank is used
+        b[i, :, r:] = float("nan")
+        for p in range(3):
+            a[i, p * 8 + r:p * 8 + 8] = float("nan")
+    want, size = lora_exact(out, x, a, b, s, ranks, ends)
+    got = out.clone()
+    ops.lora_add(got, x, a, b, *ops.build_lora_rows(slots, 3, "cpu"), ranks, ends)
+    assert ((got.double() - want).abs()
+            <= want.abs() * 2 ** -8 * 1.01 + size * 2 ** -20).all()
+    assert torch.equal(got[[1, 3, 4, 6]], out[[1, 3, 4, 6]])
+
+
+def refused_products(device):
+    q = torch.zeros(4, 64, dtype=E4M3, device=device)
+    w = torch.zeros(16, 64, dtype=E4M3, device=device)
+    s, t = torch.ones(4, device=device), torch.ones(16, device=device)
+    bias = torch.zeros(16, dtype=torch.bfloat16, device=device)
+    ops.linear_fp8(q, s, w, t, bias)
+    return [lambda: ops.linear_fp8(q[:, :40].contiguous(), s, w[:, :40].contiguous(), t),
+            lambda: ops.linear_fp8(q, s, w[:12], t[:12]),
+            lambda: ops.linear_fp8(q, s[:3], w, t),
+            lambda: ops.linear_fp8(q, s, w, t[:8]),
+            lambda: ops.linear_fp8(q, s, w[:, :32].contiguous(), t),
+            lambda: ops.linear_fp8(q, s, w, t, bias[:8]),
+            lambda: ops.linear_fp8(q.float().bfloat16(), s, w, t)]
+
+
+def refused_rows(device):
+    x = torch.zeros(2, 64, dtype=torch.bfloat16, device=device)
+    w = torch.zeros(64, dtype=torch.bfloat16, device=device)
+    wide = torch.zeros(1, 65544, dtype=torch.bfloat16, device=device)
+    return [lambda: ops.rows_fp8(x[:, :60]),
+            lambda: ops.rows_fp8(wide),
+            lambda: ops.silu_and_mul_fp8(x[:, :40].contiguous()),
+            lambda: ops.add_rms_norm_fp8(x, x[:1], w, 1e-5),
+            lambda: ops.add_rms_norm_fp8(x, None, w[:32], 1e-5)]
+
+
+def refused_adapters(device):
+    ends = (16, 24)
+    parts = lora_case(5, 32, ends, 2, 8, [0, 1, 1, 0, -1], [8, 8], 1)
+    out, x, a, b, _, ranks = (t.to(device) for t in parts)
+    order, starts = ops.build_lora_rows([0, 1, 1, 0, -1], 2, device)
+    good = dict(out=out, x=x, a=a, b=b, order=order, starts=starts, ranks=ranks,
+                ends=ends)
+    ops.lora_add(**good)
+    bad = [dict(ends=(16,)), dict(ends=(16, 20)), dict(ends=(24, 24)), dict(ends=()),
+           dict(a=a[:, :8].contiguous()), dict(b=b[:1]), dict(x=x[:4]),
+           dict(x=x[:, :24].contiguous()), dict(out=out[:, :16].contiguous()),
+           dict(starts=starts[:2]), dict(ranks=ranks[:1]),
+           dict(order=torch.cat([order, order])),
+           dict(a=a[:, :8].contiguous(), b=b[:, :, :4].contiguous())]
+    return [lambda c=c: ops.lora_add(**(good | c)) for c in bad]
+
+
+@pytest.mark.parametrize("which", [refused_products, refused_rows, refused_adapters])
+def test_refusals(which):
+    for i, call in enumerate(which("cpu")):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was taken")

@@ -1,0 +1,333 @@
+"""The kernels of rows in 8 bits, their products and adapters beside a projection
+against 64-bit forms."""
+import pytest
+import torch
+
+from gpustack_amd import ops
+from test_fp8_lora import (E4M3, lora_case, lora_exact, refused_adapters,
+                           refused_products, refused_rows)
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+
+
+def _randn(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)
+                       ).bfloat16()
+
+
+def _check_rows(r, v, slack):
+    """q s is v to within half a step of e4m3, and `slack` of the row's fp32
+    arithmetic relative to v."""
+    v = v.double().cpu()
+    q, s = r.q.cpu().double(), r.scale.cpu().double()
+    top = v.abs().amax(1)
+    assert ((s - (top / 448).clamp(min=2. ** -100)).abs() <= s * (slack + 2 ** -22)).all()
+    half = torch.maximum(v.abs() * 2 ** -4, s[:, None] * 2 ** -10)
+    assert ((q * s[:, None] - v).abs() <= half * (1 + 2 ** -19) + v.abs() * slack
+            + top[:, None] * 2. ** -22).all()
+
+
+WIDTHS = [8, 504, 512, 520, 1024, 2048, 2056, 4096, 5120, 8192, 8200, 14336, 16392,
+          32776, 65536]
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("rows", [1, 5])
+def test_rows(width, rows):
+    x = _randn(rows, width, seed=width).cuda()
+    _check_rows(ops.rows_fp8(x), x, 0)
+    g = _randn(rows, 2 * width, seed=width + 1).cuda() * 3
+    d = g.double()
+    v = d[:, :width] * torch.sigmoid(d[:, :width]) * d[:, width:]
+    # over_one_plus_exp is within 1.34e-7 of the quotient, a product behind it
+    _check_rows(ops.silu_and_mul_fp8(g), v, 2 ** -21)
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("rows,keep,residual", [(1, False, True), (5, True, True),
+                                                (6, True, False)])
+def test_norm(width, rows, keep, residual):
+    x, res = _randn(rows, width, seed=1).cuda(), _randn(rows, width, seed=2).cuda()
+    w = _randn(width, seed=3).cuda()
+    before = x.clone(), res.clone()
+    r, total = ops.add_rms_norm_fp8(x, res if residual else None, w, 1e-5, rows=keep)
+    want = (x.float() + res.float()).bfloat16() if residual else x
+    assert torch.equal(total, want)
+    assert torch.equal(x, before[0]) and torch.equal(res, before[1])
+    t = want.double()
+    v = t * (t.square().mean(1, keepdim=True) + 1e-5) ** -.5 * w.double()
+    # the sum of width squares in fp32: of 8 NV neighbours, a wave's 6 steps, 16 waves
+    slack = (64 + 6 + 16 + 6) * 2. ** -24
+    _check_rows(r, v, slack)
+    assert (r.rows is not None) == keep
+    if keep:
+        assert ((r.rows.double() - v).abs() <= v.abs() * (2 ** -8 + 2 * slack)).all()
+
+
+def test_rows_of_a_slice_and_without_numbers():
+    base = _randn(9, 4096, seed=5).cuda()
+    x = base[1::2, 1024:1544]                  # rows of 520 of stride 8192
+    a, b = ops.rows_fp8(x), ops.rows_fp8(x.contiguous())
+    assert torch.equal(a.q.float(), b.q.float()) and torch.equal(a.scale, b.scale)
+    v = torch.zeros(5, 5120, dtype=torch.bfloat16)
+    v[1, 3000], v[2, 5119], v[3, 0] = float("inf"), float("nan"), 2.0 ** -120
+    v[4] = _randn(5120, seed=6)
+    got, want = ops.rows_fp8(v.cuda()), ops.rows_fp8(v)
+    assert torch.equal(got.scale.cpu().nan_to_num(nan=7), want.scale.nan_to_num(nan=7))
+    q, p = got.q.cpu().float(), want.q.float()
+    assert torch.equal(q[:2].nan_to_num(nan=7), p[:2].nan_to_num(nan=7))
+    assert torch.isnan(q[2]).all() and (q[3] == 0).all()
+    y = ops.linear_fp8(got.q, got.scale, torch.ones(8, 5120, device="cuda").to(E4M3),
+                       torch.ones(8, device="cuda")).cpu()
+    assert (y[0] == 0).all() and torch.isnan(y[1]).all() and torch.isnan(y[2]).all()
+    assert torch.isfinite(y[3:]).all()         # a row's faults stay its own
+
+
+PRODUCTS = [(1, 8, 16), (1, 4096, 256), (3, 48, 272), (16, 72, 4096), (16, 6144, 1040),
+            (17, 8, 128), (17, 264, 144), (32, 4096, 512), (33, 128, 2064),
+            (64, 1032, 1024), (65, 512, 784), (100, 2048, 11008), (128, 24, 96),
+            (129, 136, 4096), (257, 520, 1296), (300, 1536, 128), (511, 4104, 256),
+            (700, 1024, 4160), (1031, 2568, 640)]
+
+
+def product_case(M, N, K, seed):
+    q = _randn(M, K, seed=seed).float().to(E4M3)
+    w = _randn(N, K, seed=seed + 1).float().to(E4M3)
+    s = torch.rand(M, generator=torch.Generator().manual_seed(seed)) + .1
+    t = torch.rand(N, generator=torch.Generator().manual_seed(seed + 1)) + .1
+    return q, s, w, t
+
+
+def check_product(y, q, s, w, t, bias=None):
+    """A bf16 rounding, the fp32 sums of products in sixteenths of K and more, the
+    scales, and what the matrix unit drops: of 8 neighbouring products it cuts each at
+    2^-13 of the power of two of the largest (seen with 2^16 - 2^16 + 1.5, which is 0
+    where the three are neighbours, and 1.5 elsewhere), so 7 of them lose less than
+    7 2^-13 of the largest, which is at most the product of both sides' largest. That
+    bound lets every cut fall on the same side; as they do not, all errors together
+    are within a bf16 rounding of all results."""
+    q, s, w, t = q.cuda().double(), s.cuda().double(), w.cuda().double(), t.cuda().double()
+    st = s[:, None] * t
+    want, size = q @ w.T * st, q.abs() @ w.abs().T * st
+    top = lambda v: v.abs().unflatten(1, (-1, 8)).amax(2)
+    cut = top(q) @ top(w).T * st * 7 * 2 ** -13
+    if bias is not None:
+        want, size = want + bias.cuda().double(), size + bias.cuda().double().abs()
+    K = q.shape[1]
+    off = (y.double() - want).abs()
+    assert (off <= want.abs() * 2 ** -8 + cut + size * (K / 16 + 16) * 2 ** -23).all()
+    assert off.norm() <= want.norm() * 2 ** -8
+
+
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_product(M, N, K):
+    q, s, w, t = product_case(M, N, K, M + N + K)
+    dev = [v.cuda() for v in (q, s, w, t)]
+    check_product(ops.linear_fp8(*dev), q, s, w, t)
+    bias = _randn(N, seed=9)
+    check_product(ops.linear_fp8(*dev, bias.cuda()), q, s, w, t, bias)
+
+
+def test_product_of_no_rows():
+    q, s, w, t = (v.cuda() for v in product_case(2, 16, 64, 0))
+    assert ops.linear_fp8(q[:0], s[:0], w, t).shape == (0, 16)
+    assert ops.rows_fp8(torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+                        ).q.shape == (0, 64)
+
+
+def check_lora(case, ends, order_slots=None, strides=(0, 0)):
+    out, x, a, b, slots, ranks = case
+    S, N, R = b.shape
+    for i, r in enumerate(ranks.tolist()):     # nothing behind the rank is used
+        b[i, :, r:] = float("nan")
+        for p in range(len(ends)):
+            a[i, p * R + r:(p + 1) * R] = float("nan")
+    want, size = lora_exact(out, x, a, b, slots, ranks, ends)
+
+    def rows(v, more):
+        wide = torch.full((v.shape[0], v.shape[1] + more), 3.0, dtype=v.dtype)
+        wide[:, more // 2:more // 2 + v.shape[1]] = v
+        wide = wide.cuda()
+        return wide, wide[:, more // 2:more // 2 + v.shape[1]]
+
+    whole, got = rows(out, strides[0])
+    ops.lora_add(got, rows(x, strides[1])[1], a.cuda(), b.cuda(),
+                 *ops.build_lora_rows(slots.tolist(), S, "cuda"), ranks.cuda(), ends)
+    K = x.shape[1]
+    # one rounding; h in two bf16 parts; fp32 sums over k and over the rank
+    bound = want.abs() * 2 ** -8 + size * (2 ** -16 + (K / 16 + R + 16) * 2. ** -23)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+    none = (slots < 0) | (slots >= S)
+    assert torch.equal(got.cpu()[none], out[none])
+    if strides[0]:                             # nothing beside the rows is written
+        half = strides[0] // 2
+        assert (whole[:, :half] == 3).all() and (whole[:, -half:] == 3).all()
+
+
+ADAPTERS = [  # rows, K, ends, slots, R, kind of batch
+    (1, 64, (64,), 1, 8, "one"), (1, 4096, (4096, 5120, 6144), 4, 16, "one"),
+    (3, 72, (8, 264), 2, 16, "steps"), (17, 520, (48,), 5, 24, "steps"),
+    (64, 1024, (1000, 2000), 32, 64, "steps"), (33, 256, (256, 512, 776, 1040), 70, 40,
+                                                "steps"),
+    (40, 192, (304,), 3, 256, "steps"), (5, 128, (136,), 200, 128, "steps"),
+    (300, 320, (256, 320), 3, 32, "prompts"), (257, 1000, (520,), 2, 72, "prompts"),
+    (1000, 136, (96, 192, 392), 7, 16, "prompts"), (511, 512, (640,), 1, 136, "prompts"),
+    (200, 64, (72,), 2, 256, "prompts")]
+
+
+def _slots(T, S, kind, seed):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "one":
+        return [S - 1] * T
+    if kind == "steps":
+        return torch.randint(-1, S + 1, (T,), generator=g).tolist()
+    cuts = torch.randint(0, T, (2 * S,), generator=g).sort().values
+    of = torch.randint(-1, S, (2 * S + 1,), generator=g)
+    return of[torch.bucketize(torch.arange(T), cuts, right=True)].tolist()
+
+
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("T,K,ends,S,R,kind", ADAPTERS)
+def test_adapters(T, K, ends, S, R, kind, mixed):
+    g = torch.Generator().manual_seed(T)
+    ranks = torch.randint(0, R + 1, (S,), generator=g).tolist() if mixed else [R] * S
+    case = lora_case(T, K, ends, S, R, _slots(T, S, kind, T + S), ranks, T + K)
+    check_lora(case, ends, strides=(16, 32) if mixed else (0, 0))
+
+
+def test_adapters_of_faulty_rows_and_lists():
+    """A row without numbers is that row's; entries that name no row are passed
+    over; lists beyond the order are cut."""
+    ends = (64, 128)
+    slots = [0, 1, 0, 1, -1, 0]
+    case = lora_case(6, 96, ends, 2, 16, slots, [16, 16], 4)
+    out, x, a, b, _, ranks = (t.cuda() for t in case)
+    order, starts = ops.build_lora_rows(slots, 2, "cuda")
+    want = out.clone()
+    ops.lora_add(want, x, a, b, order, starts, ranks, ends)
+    bad, got = x.clone(), out.clone()
+    bad[2] = float("nan")
+    ops.lora_add(got, bad, a, b, order, starts, ranks, ends)
+    assert torch.isnan(got[2]).all()
+    keep = [0, 1, 3, 4, 5]
+    assert torch.equal(got[keep], want[keep])
+    got = out.clone()
+    holes = order.clone()
+    holes[order == 2] = 77
+    holes[order == 3] = -5
+    ops.lora_add(got, x, a, b, holes, starts, ranks, ends)
+    assert torch.equal(got[[2, 3]], out[[2, 3]])
+    assert torch.equal(got[[0, 1, 5]], want[[0, 1, 5]])
+    got = out.clone()
+    far = starts.clone()
+    far[1:] = 1000                             # slot 0 has all there is
+    ops.lora_add(got, x, a, b, order, far, ranks, ends)
+    one = out.clone()
+    ops.lora_add(one, x, a, b, *ops.build_lora_rows([0] * 6, 2, "cuda"), ranks, ends)
+    assert torch.equal(got, one)
+
+
+@pytest.mark.parametrize("which", [refused_products, refused_rows, refused_adapters])
+def test_refusals(which):
+    for i, call in enumerate(which("cuda")):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_refusals_of_places():
+    """Operands at odd addresses, of other strides or on the CPU."""
+    q, s, w, t = (v.cuda() for v in product_case(4, 16, 64, 0))
+    x = _randn(4, 65).cuda()
+    odd = torch.zeros(4 * 64 + 1, dtype=torch.uint8, device="cuda")[1:].view(E4M3).view(4, 64)
+    for call in (lambda: ops.linear_fp8(odd, s, w, t),
+                 lambda: ops.linear_fp8(q.T.contiguous().T, s, w, t),
+                 lambda: ops.linear_fp8(q, s, w.cpu(), t),
+                 lambda: ops.linear_fp8(q, s.double(), w, t),
+                 lambda: ops.linear_fp8(q, s, w, t, dtype=torch.float32),
+                 lambda: ops.rows_fp8(x[:, 1:]),
+                 lambda: ops.rows_fp8(x[:, :64]),
+                 lambda: ops.rows_fp8(x[:, :64].float().contiguous())):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail("taken")
+
+
+def _layer(x, res, norm, w, t, a, b, order, starts, ranks, ends):
+    """A projection as a layer has it: norm, product, adapters."""
+    r, total = ops.add_rms_norm_fp8(x, res, norm, 1e-5, rows=True)
+    y = ops.linear_fp8(r.q, r.scale, w, t)
+    ops.lora_add(y, r.rows, a, b, order, starts, ranks, ends)
+    return y, total
+
+
+def _layer_case(T, K, ends, S, R, seed):
+    _, x, a, b, _, ranks = lora_case(T, K, ends, S, R, [0] * T, [R] * S, seed)
+    _, _, w, t = product_case(1, ends[-1], K, seed)
+    t = t * K ** -.5
+    res, norm = _randn(T, K, seed=seed + 5), _randn(K, seed=seed + 6)
+    return [v.cuda() for v in (x, res, norm, w, t, a, b)], ranks.cuda()
+
+
+@pytest.mark.parametrize("T", [1, 7, 130])
+def test_layer_together(T):
+    ends = (256, 320, 384)
+    slots = _slots(T, 3, "steps", T)
+    (x, res, norm, w, t, a, b), ranks = _layer_case(T, 512, ends, 3, 16, T)
+    lists = ops.build_lora_rows(slots, 3, "cuda")
+    y, total = _layer(x, res, norm, w, t, a, b, *lists, ranks, ends)
+    v = total.double()
+    h = v * (v.square().mean(1, keepdim=True) + 1e-5) ** -.5 * norm.double()
+    # the 8-bit rows are within half a step, 2^-4, of the norm's, or 2^-10 of their scale
+    weights = w.double() * t.double()[:, None]
+    off = torch.maximum(h.abs() * 2 ** -4, h.abs().amax(1, keepdim=True) / 448 * 2 ** -10)
+    want, size = lora_exact((h @ weights.T).cpu(), h.cpu(), a.cpu(), b.cpu(),
+                            torch.tensor(slots), ranks.cpu(), ends)
+    base = (h @ weights.T).cpu()
+    # two bf16 roundings, of the product and of the sum; the rows' bf16 rounding
+    bound = (off @ weights.abs().T).cpu() * (1 + 2 ** -10) \
+        + (base.abs() + want.abs()) * (2 ** -8 + 2 ** -15) + size * (2 ** -8 + 2 ** -12)
+    assert ((y.cpu().double() - want).abs() <= bound).all()
+
+
+def test_captured_layers_share_nothing():
+    """Two captured projections, replayed in turn with eager work between, other
+    lists and rows in their static buffers each time."""
+    ends, S = (128, 256), 3
+    made = []
+    for T in (6, 70):
+        parts, ranks = _layer_case(T, 256, ends, S, 16, T)
+        order, starts = ops.build_lora_rows(_slots(T, S, "steps", T), S, "cuda")
+        args = (*parts, order, starts, ranks, ends)
+        _layer(*args)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _layer(*args)
+        made.append((T, args, graph, out))
+    for turn in range(4):
+        for T, args, graph, out in made:
+            args[0].copy_(_randn(T, 256, seed=turn * 10 + T))
+            order, starts = ops.build_lora_rows(_slots(T, S, "steps", turn), S, "cuda")
+            args[7].copy_(order)
+            args[8].copy_(starts)
+        for T, args, graph, out in made:
+            graph.replay()
+        for T, args, graph, out in made:
+            want = _layer(*args)
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_another_stream():
+    ends = (256,)
+    parts, ranks = _layer_case(40, 512, ends, 2, 32, 1)
+    lists = ops.build_lora_rows(_slots(40, 2, "steps", 1), 2, "cuda")
+    want = _layer(*parts, *lists, ranks, ends)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = _layer(*parts, *lists, ranks, ends)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
