@@ -1994,21 +1994,13 @@ class Rows8(NamedTuple):
     rows: torch.Tensor | None = None   # [T, H]
 
 
-def _rows8(x, width: int) -> Rows8:
-    return Rows8(torch.empty(x.shape[0], width, dtype=torch.float8_e4m3fn,
-                             device=x.device),
-                 torch.empty(x.shape[0], dtype=torch.float32, device=x.device))
-
-
 def rows_fp8(x) -> Rows8:
     """x [T, H] in 8 bits (torch_ref.fp8_rows has the semantics). On the GPU
     bf16, rows of any stride that keeps them at multiples of 16 bytes."""
     k = _fp8_backend(x)
     if k is None:
         return Rows8(*torch_ref.fp8_rows(x))
-    r = _rows8(x, x.shape[1])
-    k.fp8_rows(0, r.q, r.scale, None, None, x, None, None, 0.0)
-    return r
+    return Rows8(*k.fp8_rows(0, x, None, None, 0.0, False)[:2])
 
 
 def silu_and_mul_fp8(x) -> Rows8:
@@ -2016,9 +2008,7 @@ def silu_and_mul_fp8(x) -> Rows8:
     k = _fp8_backend(x)
     if k is None:
         return Rows8(*torch_ref.silu_and_mul_fp8(x))
-    r = _rows8(x, x.shape[1] // 2)
-    k.fp8_rows(1, r.q, r.scale, None, None, x, None, None, 0.0)
-    return r
+    return Rows8(*k.fp8_rows(1, x, None, None, 0.0, False)[:2])
 
 
 def add_rms_norm_fp8(x, residual, weight, eps: float, rows: bool = False):
@@ -2030,20 +2020,97 @@ def add_rms_norm_fp8(x, residual, weight, eps: float, rows: bool = False):
     if k is None:
         q, scale, h, total = torch_ref.add_rms_norm_fp8(x, residual, weight, eps)
         return Rows8(q, scale, h if rows else None), total
-    r = _rows8(x, x.shape[1])
-    like = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = like() if residual is not None else None
-    h = like() if rows else None
-    k.fp8_rows(2, r.q, r.scale, total, h, x, residual, weight, eps)
-    return Rows8(r.q, r.scale, h), x if total is None else total
+    q, scale, total, h = k.fp8_rows(2, x, residual, weight, eps, rows)
+    return Rows8(q, scale, h), x if total is None else total
 
 
+# Times of an 8-bit product's kernels in us, by 16 rows and columns of a workgroup
+# (fp8_rows_gemm_kernel), 16 rows and columns of a tile (fp8_tile_kernel), 32 of them
+# (fp8_wide_kernel): the launch, a round, a round's step, a step's share of all the
+# steps over the CUs, a MB of weights, a join, a MB of its parts (of the first: a round's
+# step and row), a MB of the result. Fitted to 8126 sizes (1 to 8192 rows, 512 to 28672
+# columns, 512 to 15360 k, weights out of HBM), off by 5 to 10 % of a time; the least by
+# them costs 2 % more than the best on average, 5 % in one size of six.
+_FP8_ROWS = {
+    (1, 16): (2.27, .351, .798, 0, .164, .037, 1.00, .01),
+    (1, 32): (2.09, .174, 1.71, .177, .173, .034, 4.04, .711),
+    (2, 16): (1.89, .601, .656, 0, .168, .05, 1.00, 0),
+    (2, 32): (1.61, .924, 1.51, .074, .181, .052, 1.76, .339),
+    (4, 16): (1.79, .999, 1.43, 0, .285, .034, 1.00, .202)}
+_FP8_TILES = {
+    (2, 2): (1.25, 1.63, .158, .045, .181, 3.47, 1.33, 0),
+    (2, 4): (1.58, 1.27, .118, .13, .173, 3.34, 1.03, 0),
+    (2, 8): (2.26, 1.13, 0, .372, .172, 2.52, 1.13, .05),
+    (4, 2): (2.31, .298, .256, .019, .215, 2.85, 1.63, .148),
+    (4, 4): (2.82, .344, .217, .122, .157, 2.33, 1.44, .077),
+    (4, 8): (4.04, 0, .039, .424, .138, 1.43, 1.51, .024),
+    (8, 2): (2.60, .441, .295, .104, .283, 2.15, 1.60, .198),
+    (8, 4): (4.01, 0, .144, .316, .188, 1.36, 1.57, .185),
+    (8, 8): (5.73, .178, .415, .215, .157, 0, 1.49, .202)}
+_FP8_WIDE = {
+    (4, 2): (3.12, .798, .255, .064, .247, 2.40, 2.10, .072),
+    (4, 4): (3.56, .925, .346, .134, .209, 2.69, 1.84, .1),
+    (4, 6): (4.05, .828, .464, .176, .184, 3.14, 1.58, .139),
+    (4, 8): (4.44, .519, .57, .25, .182, 3.54, 1.40, .151),
+    (6, 6): (3.56, 1.71, .606, .19, .166, 3.52, 1.40, .15),
+    (6, 8): (3.29, 2.67, .757, .225, .175, 4.01, 1.25, .151),
+    (8, 4): (4.18, .954, .546, .192, .147, 3.02, 1.58, .189),
+    (8, 6): (3.48, 2.51, .734, .221, .126, 3.59, 1.29, .184),
+    (8, 8): (3.18, 3.82, .928, .234, .159, 3.86, 1.22, .174)}
+# workgroups of a tile that a CU holds
+_FP8_HELD = {(2, 2): 5, (2, 4): 3, (2, 8): 2, (4, 2): 3, (4, 4): 2, (4, 8): 2,
+             (8, 2): 2, (8, 4): 2, (8, 8): 1}
+
+
+def _fp8_time(kind: int, a: int, b: int, splits: int, M: int, N: int, K: int):
+    steps = -(-K // 128)
+    if kind == 0:
+        p = _FP8_ROWS[a, b]
+        n = -(-N // b)
+        rounds, each = -(-n // 256), -(-K // 2048)
+        share, moved, joins, parts = each * n / 256, N * K, each * M * rounds, 0
+        held = each * rounds
+    else:
+        p = _FP8_TILES[a, b] if kind == 1 else _FP8_WIDE[a, b]
+        rows = (16 if kind == 1 else 32) * a
+        down = -(-M // rows)
+        n = down * -(-N // (rows // a * b)) * splits
+        each = -(-steps // splits) if kind == 1 else 2 * -(-((steps + 1) // 2) // splits)
+        rounds = -(-n // (256 * (_FP8_HELD[a, b] if kind == 1 else 1)))
+        share = each * (-(-n // 256) if kind == 1 else n / 256)
+        moved = N * K * (down if kind == 1 else 1)
+        joins, parts = (1, splits * M * N / 1e6) if splits > 1 else (0, 0)
+        held = each * rounds
+    work = p[0] + rounds * p[1] + held * p[2] + share * p[3]
+    memory = p[0] + moved / 1e6 * p[4]
+    return (work ** 6 + memory ** 6) ** (1 / 6) + joins * p[5] + parts * p[6] \
+        + 2 * M * N / 1e6 * p[7]
+
+
+@functools.lru_cache(maxsize=8192)
 def _fp8_plan(M: int, N: int, K: int):
-    """(rows, columns of a tile in 16, parts over k) of an 8-bit product."""
-    mt = 2 if M <= 32 else 4 if M <= 64 else 8
-    nt = 8
-    tiles = -(-M // (16 * mt)) * -(-N // (16 * nt))
-    return mt, nt, max(1, min(512 // tiles, -(-K // 1024)))
+    """(kind, a, b, parts over k) of the least time (_fp8_time) of an 8-bit product:
+    0 straight from memory, up to 64 rows; 1 tiles of up to 128 rows, up to 300; 2
+    tiles of up to 256 rows by persistent workgroups, from 65, whose offsets are 32 bits
+    (31 where rows end within a step)."""
+    plans = []
+    if M <= 64:
+        plans += [(0, a, b, 1) for a, b in _FP8_ROWS
+                  if M <= 16 * a and (a == 1 or M > 8 * a)]
+    wide = (M > 64 and K >= 128 and (N + 256) * K < 1 << (31 if K % 128 else 32)
+            and K < 1 << 22 and N < 1 << 21)
+    if M <= 300 or not wide:
+        plans += [(1, a, b, s) for a, b in _FP8_TILES for s in (1, 2, 3, 4, 6, 8, 12)
+                  if (a == 2 or M > 8 * a) and (M <= 32 * a or a == 8)
+                  and (s == 1 or s * 256 <= K and -(-M // (16 * a)) * -(-N // (16 * b)) * s
+                       <= 1024 and s * M * N < 1 << 28)]
+    if wide:
+        for a, b in _FP8_WIDE:
+            n = -(-M // (32 * a)) * -(-N // (32 * b))
+            fill = 256 // n
+            plans += [(2, a, b, s) for s in {1, 2, 3, 4, fill // 2, fill}
+                      if s == 1 or 1 < s <= min(fill + 1, 16) and s * 512 <= K]
+    return min(plans, key=lambda p: (_fp8_time(*p, M, N, K), p))
 
 
 def linear_fp8(q, scale, w, w_scale, bias=None, dtype=torch.bfloat16):
@@ -2053,13 +2120,10 @@ def linear_fp8(q, scale, w, w_scale, bias=None, dtype=torch.bfloat16):
     k = _fp8_backend(q)
     if k is None:
         return torch_ref.linear_fp8(q, scale, w, w_scale, bias, dtype)
-    M, N = q.shape[0], w.shape[0]
-    out = torch.empty(M, N, dtype=dtype, device=q.device)
-    if M <= 16:
-        k.fp8_rows_gemm(out, q, scale, w, w_scale, bias, 16)
-    else:
-        k.fp8_tile(out, q, scale, w, w_scale, bias, *_fp8_plan(M, N, q.shape[1]))
-    return out
+    if dtype != torch.bfloat16 or q.dim() != 2 or w.dim() != 2:
+        raise RuntimeError("fp8 product: x [M, K] and w [N, K] to bf16")
+    return k.fp8_linear(q, scale, w, w_scale, bias,
+                        *_fp8_plan(q.shape[0], w.shape[0], q.shape[1]))
 
 
 def build_lora_rows(slots, n_slots: int, device):

@@ -24,7 +24,8 @@ HEADERS = ["common.h", "wide_tiles.h", "pinned_words.h"]
 # the fp32-residual op family lives in its own small library: a checkout
 # that serves only such a model compiles these few files and nothing else
 LATENT_SO_PATH = PKG_DIR / "_hip_latent.so"
-SMALL_HEADERS = ["common.h", "short_conv_binding.h", "pinned_words.h"]
+SMALL_HEADERS = ["common.h", "short_conv_binding.h", "pinned_words.h",
+                 "wide_tiles.h"]
 LATENT_SOURCES = ["resid32.hip", "latent_attn.hip", "grouped_ff.hip",
                   "latent_bindings.cpp"]
 
@@ -51,7 +52,8 @@ STREAMS_SOURCES = ["hyperrows32.hip", "gru_scan.hip", "short_conv.hip",
 
 # rows in 8 bits, their products, adapters beside a projection
 FP8_SO_PATH = PKG_DIR / "_hip_fp8.so"
-FP8_SOURCES = ["fp8_rows.hip", "fp8_gemm.hip", "lora.hip", "fp8_bindings.cpp"]
+FP8_SOURCES = ["fp8_rows.hip", "fp8_gemm.hip", "fp8_wide.hip", "lora.hip",
+               "fp8_bindings.cpp"]
 
 
 def _torch_paths():

@@ -8,9 +8,12 @@
 
 int fp8_rows_most();
 void fp8_rows_launch(int, void*, float*, void*, void*, const void*, long, const void*, const void*, float, int, int, hipStream_t);
-void fp8_rows_gemm_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, hipStream_t);
+void fp8_rows_gemm_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, hipStream_t);
+bool fp8_rows_has(int, int);
 bool fp8_tile_has(int, int);
-void fp8_tile_launch(void*, void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, int, hipStream_t);
+void fp8_tile_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, int, hipStream_t);
+void fp8_join_launch(void*, const void*, const float*, const float*, const void*, int, int, int, hipStream_t);
+void fp8_wide_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, int, int*, hipStream_t);
 int lora_most_rank();
 void lora_launch(void*, long, float*, const void*, long, const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, const int*, int, int, int, hipStream_t);
 
@@ -54,51 +57,53 @@ long chk_rows(const Tensor& t, const char* name, const Tensor& like) {
   return stride;
 }
 
-void fp8_rows(int64_t source, Tensor q, Tensor scale, OptTensor sum, OptTensor rows,
-              Tensor x, OptTensor residual, OptTensor weight, double eps) {
-  TORCH_CHECK(source >= 0 && source <= 2, "fp8_rows: no such source");
+// (q, scale, sum, rows): source 0 x as it is, 1 silu(gate) * up, 2 the norm of
+// x + residual, whose sum comes too, or of x; `keep`: the norm in bf16 as well
+std::tuple<Tensor, Tensor, OptTensor, OptTensor> fp8_rows(
+    int64_t source, Tensor x, OptTensor residual, OptTensor weight, double eps,
+    bool keep) {
   const long xs = chk_rows(x, "x", x);
   const long T = x.size(0), W = x.size(1), H = source == 1 ? W / 2 : W;
+  TORCH_CHECK(source >= 0 && source <= 2, "fp8_rows: no such source");
   TORCH_CHECK(T < 1l << 31 && H >= 8 && H % 8 == 0 && H <= fp8_rows_most() &&
               (source != 1 || W % 2 == 0),
               "fp8_rows: rows of ", W, " elements: the result's are a multiple of 8, at most ",
               fp8_rows_most());
-  chk(q, "q", at::kFloat8_e4m3fn, x);
-  chk(scale, "scale", at::kFloat, x);
-  TORCH_CHECK(q.dim() == 2 && q.size(0) == T && q.size(1) == H && scale.dim() == 1 &&
-              scale.size(0) == T, "fp8_rows: shapes of the result");
-  TORCH_CHECK(residual.has_value() == sum.has_value(), "fp8_rows: residual and its sum");
-  TORCH_CHECK(weight.has_value() == (source == 2) && (source == 2 || !(residual || rows)),
+  TORCH_CHECK(weight.has_value() == (source == 2) && (source == 2 || !(residual || keep)),
               "fp8_rows: what belongs to the norm");
   if (weight) {
     chk(*weight, "weight", at::kBFloat16, x);
     TORCH_CHECK(weight->dim() == 1 && weight->size(0) == H, "fp8_rows: weight's size");
   }
-  for (const auto& t : {std::make_pair(&residual, "residual"), std::make_pair(&sum, "sum"),
-                        std::make_pair(&rows, "rows")})
-    if (t.first->has_value()) {
-      chk(**t.first, t.second, at::kBFloat16, x);
-      TORCH_CHECK((*t.first)->dim() == 2 && (*t.first)->size(0) == T &&
-                  (*t.first)->size(1) == H, "fp8_rows: shape of ", t.second);
-    }
-  if (T == 0) return;
+  if (residual) {
+    chk(*residual, "residual", at::kBFloat16, x);
+    TORCH_CHECK(residual->sizes() == x.sizes(), "fp8_rows: shape of residual");
+  }
   const at::DeviceGuard guard(x.device());
-  auto at = [](const OptTensor& t) { return t ? t->data_ptr() : nullptr; };
-  fp8_rows_launch((int)source, q.data_ptr(), scale.data_ptr<float>(), at(sum), at(rows),
-                  x.data_ptr(), xs, at(residual), at(weight), (float)eps, (int)T, (int)H,
-                  cur_stream(x));
-  HIP_CHECK_LAST();
+  Tensor q = at::empty({T, H}, x.options().dtype(at::kFloat8_e4m3fn));
+  Tensor scale = at::empty({T}, x.options().dtype(at::kFloat));
+  OptTensor sum, rows;
+  if (residual) sum = at::empty({T, H}, x.options());
+  if (keep) rows = at::empty({T, H}, x.options());
+  if (T > 0) {
+    auto at = [](const OptTensor& t) { return t ? t->data_ptr() : nullptr; };
+    fp8_rows_launch((int)source, q.data_ptr(), scale.data_ptr<float>(), at(sum), at(rows),
+                    x.data_ptr(), xs, at(residual), at(weight), (float)eps, (int)T, (int)H,
+                    cur_stream(x));
+    HIP_CHECK_LAST();
+  }
+  return {q, scale, sum, rows};
 }
 
-struct Product { int M, N, K; const void* bias; };
-
-Product chk_product(const Tensor& out, const Tensor& x, const Tensor& xs, const Tensor& w,
-                    const Tensor& ws, const OptTensor& bias) {
+// The product by the plan that the caller chose: kind 0 straight from memory (16 a
+// rows, b columns a workgroup), 1 tiles of 16 a rows and 16 b columns, 2 of 32 a and
+// 32 b, these two with k in `splits` parts.
+Tensor fp8_linear(Tensor x, Tensor xs, Tensor w, Tensor ws, OptTensor bias, int64_t kind,
+                  int64_t a, int64_t b, int64_t splits) {
   chk(x, "x", at::kFloat8_e4m3fn, x);
   chk(xs, "x_scale", at::kFloat, x);
   chk(w, "w", at::kFloat8_e4m3fn, x);
   chk(ws, "w_scale", at::kFloat, x);
-  chk(out, "out", at::kBFloat16, x);
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1),
               "fp8 product: x [M, K] and w [N, K]");
   const long M = x.size(0), K = x.size(1), N = w.size(0);
@@ -107,43 +112,44 @@ Product chk_product(const Tensor& out, const Tensor& x, const Tensor& xs, const 
               "fp8 product: K a multiple of 16 and N one of 8, not ", K, " and ", N);
   TORCH_CHECK(xs.dim() == 1 && xs.size(0) == M && ws.dim() == 1 && ws.size(0) == N,
               "fp8 product: a scale a row and a scale a column");
-  TORCH_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == N,
-              "fp8 product: out [M, N]");
+  const void* bp = nullptr;
   if (bias) {
     chk(*bias, "bias", at::kBFloat16, x);
     TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N, "fp8 product: bias's size");
+    bp = bias->data_ptr();
   }
-  return {(int)M, (int)N, (int)K, bias ? bias->data_ptr() : nullptr};
-}
-
-void fp8_rows_gemm(Tensor out, Tensor x, Tensor xs, Tensor w, Tensor ws, OptTensor bias,
-                   int64_t cols) {
-  const Product p = chk_product(out, x, xs, w, ws, bias);
-  TORCH_CHECK(p.M <= 16 && (cols == 16 || cols == 32), "fp8_rows_gemm: plan");
-  if (p.M == 0) return;
   const at::DeviceGuard guard(x.device());
-  fp8_rows_gemm_launch(out.data_ptr(), x.data_ptr(), xs.data_ptr<float>(), w.data_ptr(),
-                       ws.data_ptr<float>(), p.bias, p.M, p.N, p.K, (int)cols,
-                       cur_stream(x));
-  HIP_CHECK_LAST();
-}
-
-void fp8_tile(Tensor out, Tensor x, Tensor xs, Tensor w, Tensor ws, OptTensor bias,
-              int64_t mt, int64_t nt, int64_t splits) {
-  const Product p = chk_product(out, x, xs, w, ws, bias);
-  TORCH_CHECK(fp8_tile_has(mt, nt) && splits >= 1 && splits <= (p.K + 127) / 128 &&
-              (p.N + 16 * nt - 1) / (16 * nt) * splits < 1l << 31 &&
-              p.M <= 65535l * 16 * mt,
-              "fp8_tile: plan");
-  if (p.M == 0) return;
-  const at::DeviceGuard guard(x.device());
+  Tensor out = at::empty({M, N}, x.options().dtype(at::kBFloat16));
+  if (M == 0) return out;
+  const hipStream_t s = cur_stream(x);
+  const float *sx = xs.data_ptr<float>(), *sw = ws.data_ptr<float>();
+  if (kind == 0) {
+    TORCH_CHECK(fp8_rows_has(a, b) && M <= 16 * a, "fp8 product: plan");
+    fp8_rows_gemm_launch(out.data_ptr(), x.data_ptr(), sx, w.data_ptr(), sw, bp, (int)M,
+                         (int)N, (int)K, (int)a, (int)b, s);
+    HIP_CHECK_LAST();
+    return out;
+  }
+  TORCH_CHECK((kind == 1 || kind == 2) && splits >= 1 && splits <= (K + 127) / 128 &&
+              splits <= 64, "fp8 product: plan");
   Tensor parts;
+  if (splits > 1) parts = at::empty({splits, M, N}, x.options().dtype(at::kFloat));
+  void* to = splits > 1 ? parts.data_ptr() : out.data_ptr();
+  if (kind == 1) {
+    TORCH_CHECK(fp8_tile_has(a, b) && (N + 16 * b - 1) / (16 * b) * splits < 1l << 31 &&
+                M <= 65535l * 16 * a, "fp8 product: plan");
+    fp8_tile_launch(to, x.data_ptr(), sx, w.data_ptr(), sw, bp, (int)M, (int)N, (int)K,
+                    (int)a, (int)b, (int)splits, s);
+  } else {
+    int err = 0;
+    fp8_wide_launch(to, x.data_ptr(), sx, w.data_ptr(), sw, bp, (int)M, (int)N, (int)K,
+                    (int)splits, (int)a, (int)b, &err, s);
+    TORCH_CHECK(!err, "fp8 product: plan");
+  }
   if (splits > 1)
-    parts = at::empty({splits, p.M, p.N}, x.options().dtype(at::kFloat));
-  fp8_tile_launch(out.data_ptr(), splits > 1 ? parts.data_ptr() : nullptr, x.data_ptr(),
-                  xs.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), p.bias, p.M,
-                  p.N, p.K, (int)mt, (int)nt, (int)splits, cur_stream(x));
+    fp8_join_launch(out.data_ptr(), to, sx, sw, bp, (int)M, (int)N, (int)splits, s);
   HIP_CHECK_LAST();
+  return out;
 }
 
 void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor starts,
@@ -198,7 +204,6 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_rows", &fp8_rows);
-  m.def("fp8_rows_gemm", &fp8_rows_gemm);
-  m.def("fp8_tile", &fp8_tile);
+  m.def("fp8_linear", &fp8_linear);
   m.def("lora_add", &lora_add);
 }

@@ -22,18 +22,18 @@ DEVICE_INLINE f32x4 multiply(const Bytes32& a, const Bytes32& b, const f32x4& c)
       __builtin_bit_cast(i32x8, a), __builtin_bit_cast(i32x8, b), c, 0, 0, 0, 0, 0, 0);
 }
 
-// Up to 16 rows. A workgroup of 8 waves owns 16 NTW columns; its waves take the blocks
-// of 256 k of those weight rows in turn, straight from memory, one block ahead, and
-// meet in the LDS at the end. x comes from the L2. TAIL: the last block is not whole.
+// Up to 16 MT rows. A workgroup of 8 waves owns 16 NTW columns; its waves take the
+// blocks of 256 k of those weight rows in turn, straight from memory, one block ahead
+// with the rows', and meet in the LDS at the end. x comes from the L2. TAIL: the last block is not whole.
 constexpr int FR_K = 256, FR_WAVES = 8, FR_THREADS = FR_WAVES * WAVE_SIZE;
 
-template <int NTW, bool TAIL>
+template <int MT, int NTW, bool TAIL>
 __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
     unsigned short* __restrict__ out,        // [M, N]
     const unsigned char* __restrict__ x, const float* __restrict__ xs,
     const unsigned char* __restrict__ w, const float* __restrict__ ws,
     const unsigned short* __restrict__ bias, int M, int N, int K) {
-  constexpr int COLS = 16 * NTW, ROWS = 16;
+  constexpr int COLS = 16 * NTW, ROWS = 16 * MT;
   __shared__ float red[FR_WAVES * ROWS * COLS];
   const int nb = (K + FR_K - 1) / FR_K;
   const int n0 = blockIdx.x * COLS;
@@ -45,7 +45,9 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
 #pragma unroll
   for (int t = 0; t < NTW; ++t)
     wp[t] = w + (long)min(n0 + t * 16 + lc, N - 1) * K;
-  const unsigned char* xp = x + (long)min(lc, M - 1) * K;
+  const unsigned char* xp[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xp[m] = x + (long)min(m * 16 + lc, M - 1) * K;
 
   // workgroups begin at places of their own: rows lie a power of two apart
   const int rot = blockIdx.x % nb;
@@ -60,46 +62,56 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
       return *reinterpret_cast<const u32x4*>(p + k);
     }
   };
-  u32x4 wc[NTW][4], wn[NTW][4];
-  const int b0 = block(min(wave, nb - 1));
+  u32x4 wc[NTW][4], wn[NTW][4], xc[MT][4], xn[MT][4];
+  auto fetch = [&](u32x4 (&wv)[NTW][4], u32x4 (&xv)[MT][4], int b) {
 #pragma unroll
-  for (int t = 0; t < NTW; ++t)
+    for (int t = 0; t < NTW; ++t)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) wc[t][c] = piece(wp[t], b0, c);
-  f32x4 acc[NTW];
+      for (int c = 0; c < 4; ++c) wv[t][c] = piece(wp[t], b, c);
 #pragma unroll
-  for (int t = 0; t < NTW; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) xv[m][c] = piece(xp[m], b, c);
+  };
+  fetch(wc, xc, block(min(wave, nb - 1)));
+  f32x4 acc[MT][NTW];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NTW; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto products = [&](int b) {
+  auto products = [&] {
 #pragma unroll
-    for (int c = 0; c < 4; c += 2) {
-      const Bytes32 xa{piece(xp, b, c), piece(xp, b, c + 1)};
+    for (int c = 0; c < 4; c += 2)
 #pragma unroll
-      for (int t = 0; t < NTW; ++t)
-        acc[t] = multiply(xa, Bytes32{wc[t][c], wc[t][c + 1]}, acc[t]);
-    }
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NTW; ++t)
+          acc[m][t] = multiply(Bytes32{xc[m][c], xc[m][c + 1]},
+                               Bytes32{wc[t][c], wc[t][c + 1]}, acc[m][t]);
   };
   int i = wave;
   for (; i + FR_WAVES < nb; i += FR_WAVES) {
-    const int bn = block(i + FR_WAVES);
+    fetch(wn, xn, block(i + FR_WAVES));
+    products();
 #pragma unroll
-    for (int t = 0; t < NTW; ++t)
+    for (int c = 0; c < 4; ++c) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) wn[t][c] = piece(wp[t], bn, c);
-    products(block(i));
+      for (int t = 0; t < NTW; ++t) wc[t][c] = wn[t][c];
 #pragma unroll
-    for (int t = 0; t < NTW; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) wc[t][c] = wn[t][c];
+      for (int m = 0; m < MT; ++m) xc[m][c] = xn[m][c];
+    }
   }
-  if (i < nb) products(block(i));
+  if (i < nb) products();
 
   // D[row = lg * 4 + r][column = lc] per tile
 #pragma unroll
-  for (int t = 0; t < NTW; ++t)
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      red[(wave * ROWS + lg * 4 + r) * COLS + t * 16 + lc] = acc[t][r];
+    for (int t = 0; t < NTW; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        red[(wave * ROWS + m * 16 + lg * 4 + r) * COLS + t * 16 + lc] = acc[m][t][r];
   __syncthreads();
   for (int u = tid; u < ROWS * COLS; u += FR_THREADS) {
     const int row = u / COLS, col = n0 + u % COLS;
@@ -124,9 +136,7 @@ __device__ const u32x4 fp8_zeros = {0, 0, 0, 0};
 
 template <int L>
 DEVICE_INLINE void ft_wait(int ahead) {      // all but `ahead` steps are there
-  if (ahead >= 4) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(4 * L) : "memory");
-  else if (ahead == 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(3 * L) : "memory");
-  else if (ahead == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * L) : "memory");
+  if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * L) : "memory");
   else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(L) : "memory");
   else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
@@ -139,7 +149,7 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
     const unsigned short* __restrict__ bias, int M, int N, int K, int splits) {
   constexpr int BUF = 16 * (MT + NT) * FT_K;
   constexpr int L = (MT + NT) / 2;           // loads of a wave in a step
-  static_assert(S >= 2 && S <= 6 && 4 * L <= 63 && MT % 2 == 0 && NT % 2 == 0,
+  static_assert(S >= 2 && S <= 4 && 2 * L <= 63 && MT % 2 == 0 && NT % 2 == 0,
                 "the waits above, the waves' shares");
   __shared__ __attribute__((aligned(16))) unsigned char lds[S * BUF];
   const int split = SPLIT ? blockIdx.x % splits : 0;
@@ -265,50 +275,64 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(
 
 }  // namespace
 
-// Up to 16 rows, `cols` (16 or 32) columns a workgroup. K a multiple of 16, N of 4.
+// Up to 16 mt rows, `cols` (16 or 32) columns a workgroup. K a multiple of 16, N of 4.
 void fp8_rows_gemm_launch(void* out, const void* x, const float* xs, const void* w,
                           const float* ws, const void* bias, int M, int N, int K,
-                          int cols, hipStream_t s) {
+                          int mt, int cols, hipStream_t s) {
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((N + cols - 1) / cols), dim3(FR_THREADS), 0, s,
                        (unsigned short*)out, (const unsigned char*)x, xs,
                        (const unsigned char*)w, ws, (const unsigned short*)bias, M, N, K);
   };
   const bool tail = K % FR_K != 0;
-  if (cols == 16) tail ? go(fp8_rows_gemm_kernel<1, true>) : go(fp8_rows_gemm_kernel<1, false>);
-  else tail ? go(fp8_rows_gemm_kernel<2, true>) : go(fp8_rows_gemm_kernel<2, false>);
+  switch (mt * 10 + cols / 16) {
+#define ROWS(MT, NTW)                                          \
+    case MT * 10 + NTW:                                        \
+      tail ? go(fp8_rows_gemm_kernel<MT, NTW, true>)           \
+           : go(fp8_rows_gemm_kernel<MT, NTW, false>);         \
+      break
+    ROWS(1, 1); ROWS(1, 2); ROWS(2, 1); ROWS(2, 2); ROWS(4, 1);
+#undef ROWS
+  }
+}
+
+bool fp8_rows_has(int mt, int cols) {
+  return ((mt == 1 || mt == 2) && (cols == 16 || cols == 32)) || (mt == 4 && cols == 16);
+}
+
+void fp8_join_launch(void* out, const void* parts, const float* xs, const float* ws,
+                     const void* bias, int M, int N, int splits, hipStream_t s) {
+  const long MN = (long)M * N;
+  hipLaunchKernelGGL(fp8_join_kernel, dim3((MN / 4 + 255) / 256), dim3(256), 0, s,
+                     (unsigned short*)out, (const float*)parts, xs, ws,
+                     (const unsigned short*)bias, M, N, splits);
 }
 
 bool fp8_tile_has(int mt, int nt) {
   return (mt == 2 || mt == 4 || mt == 8) && (nt == 2 || nt == 4 || nt == 8);
 }
 
-// Tiles of 16 mt rows and 16 nt columns, k in `splits` parts (fp32 [splits, M, N] each).
-void fp8_tile_launch(void* out, void* parts, const void* x, const float* xs,
-                     const void* w, const float* ws, const void* bias, int M, int N,
-                     int K, int mt, int nt, int splits, hipStream_t s) {
-  auto go = [&](auto kernel, void* to) {
+// Tiles of 16 mt rows and 16 nt columns: the product to `out`, or with k in `splits`
+// parts, more than one, those (fp32 [splits, M, N]).
+void fp8_tile_launch(void* out, const void* x, const float* xs, const void* w,
+                     const float* ws, const void* bias, int M, int N, int K, int mt,
+                     int nt, int splits, hipStream_t s) {
+  auto go = [&](auto kernel) {
     const int tiles = (N + 16 * nt - 1) / (16 * nt);
     hipLaunchKernelGGL(kernel, dim3(tiles * splits, (M + 16 * mt - 1) / (16 * mt)),
-                       dim3(256), 0, s, to, (const unsigned char*)x, xs,
+                       dim3(256), 0, s, out, (const unsigned char*)x, xs,
                        (const unsigned char*)w, ws, (const unsigned short*)bias, M, N, K,
                        splits);
   };
   switch (mt * 10 + nt) {
-#define TILE(MT, NT, S)                                              \
-    case MT * 10 + NT:                                               \
-      if (splits > 1) go(fp8_tile_kernel<MT, NT, S, true>, parts);   \
-      else go(fp8_tile_kernel<MT, NT, S, false>, out);               \
+#define TILE(MT, NT, S)                                          \
+    case MT * 10 + NT:                                           \
+      splits > 1 ? go(fp8_tile_kernel<MT, NT, S, true>)          \
+                 : go(fp8_tile_kernel<MT, NT, S, false>);        \
       break
-    TILE(2, 2, 5); TILE(2, 4, 5); TILE(2, 8, 5);
-    TILE(4, 2, 5); TILE(4, 4, 5); TILE(4, 8, 4);
-    TILE(8, 2, 4); TILE(8, 4, 4); TILE(8, 8, 4);
+    TILE(2, 2, 4); TILE(2, 4, 4); TILE(2, 8, 4);
+    TILE(4, 2, 4); TILE(4, 4, 4); TILE(4, 8, 3);
+    TILE(8, 2, 4); TILE(8, 4, 3); TILE(8, 8, 3);
 #undef TILE
-  }
-  if (splits > 1) {
-    const long MN = (long)M * N;
-    hipLaunchKernelGGL(fp8_join_kernel, dim3((MN / 4 + 255) / 256), dim3(256), 0, s,
-                       (unsigned short*)out, (const float*)parts, xs, ws,
-                       (const unsigned short*)bias, M, N, splits);
   }
 }

@@ -117,7 +117,13 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
   const float most = __builtin_bit_cast(float, top);
   // a NaN is neither below nor above the least scale, and stays
   const float s = most / TOP < LEAST ? LEAST : most / TOP;
-  const float turn = 1.f / s;
+  // the quotients as a division rounds them: by the reciprocal, put right by what that
+  // leaves, of finite scales
+  const float turn = 1.f / s, left = s < INFINITY ? turn : 0.f;
+  auto over = [&](float a) {
+    const float r = a * turn;
+    return left == 0.f ? r : __builtin_fmaf(__builtin_fmaf(-r, s, a), left, r);
+  };
   if (t == 0) scale[row] = s;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -125,10 +131,10 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
     if (c < H) {
       uint2 o;
       int lo = 0, hi = 0;
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][0] * turn, v[i][1] * turn, lo, false);
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][2] * turn, v[i][3] * turn, lo, true);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][4] * turn, v[i][5] * turn, hi, false);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[i][6] * turn, v[i][7] * turn, hi, true);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][0]), over(v[i][1]), lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][2]), over(v[i][3]), lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][4]), over(v[i][5]), hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][6]), over(v[i][7]), hi, true);
       o.x = lo;
       o.y = hi;
       *reinterpret_cast<uint2*>(q + row * H + c) = o;

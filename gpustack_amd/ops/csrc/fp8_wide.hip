@@ -1,0 +1,356 @@
+// Products of many 8-bit rows for MI355X (gfx950) in tiles of up to 256 rows and 256
+// weight rows, whole or cut over k: the e4m3 form of wide_tiles.hip, whose layout it
+// has (one persistent workgroup of four waves a CU, steps of 128 bytes of k through
+// rings of LDS buffers that are filled steps ahead and through the ends of tiles, 16-byte
+// piece c of row r at c ^ (r / 2 % 8), one LDS read or load in each gap between two
+// products, products in inline asm that add in place).
+//
+// What differs is the instruction: v_mfma_f32_16x16x128_f8f6f4 takes a whole step's 128
+// bytes of 16 rows, 8 registers a lane, so one step of 256 x 256 holds 128 registers of
+// operands and there is no room for the next one's beside it. The products of a step go
+// around a wave's four quarters instead, rows' half first, columns' half second:
+//   even steps  (0, 0) (1, 0) (1, 1) (0, 1)      odd  (1, 0) (0, 0) (0, 1) (1, 1)
+// Each quarter leaves one half of the operands free for good, and the quarter after it
+// reads that half's successor over it: the other rows and the other columns of this step
+// in the first two, the next step's columns and rows in the last two. A step's buffers
+// are read to their end before its middle, where the waves meet.
+// (Of random numbers the matrix unit does 4.1 PFLOP/s in this form before the card's
+// power limits it, 3.8 in the 32x32x64 one.)
+// Steps come in pairs; an odd number gets one of zeros. Of a step that reaches behind
+// the end of the rows, those pieces are loaded from beyond the operands: zeros, too.
+#include "wide_tiles.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+
+constexpr int FW_K = 128;
+constexpr int FW_CUS = 256;                 // workgroups of a launch
+
+template <bool PARTS, int RF, int CF>
+__global__ __launch_bounds__(256, 1) void fp8_wide_kernel(
+    void* __restrict__ out_,                // bf16 [M, N], or fp32 [splits, M, N]
+    const unsigned char* __restrict__ x, const float* __restrict__ xs,
+    const unsigned char* __restrict__ w, const float* __restrict__ ws,
+    const unsigned short* __restrict__ bias, int M, int N, int K, int splits) {
+  static_assert(RF % 2 == 0 && CF % 2 == 0, "quarters");
+  constexpr int MT = 32 * RF, WT = 32 * CF; // rows and weight rows of a tile
+  // buffers of the rows; of the weights there is one more
+  constexpr int NR = 5 * RF + 6 * CF <= 40 ? 5 : 4 * RF + 5 * CF <= 40 ? 4
+                   : 3 * RF + 4 * CF <= 40 ? 3 : 2;
+  constexpr int NW = NR + 1;
+  // loads behind the last one of the next step, halfway through a step
+  constexpr int BEHIND = CF * (NR - 1) + RF * (NR - 2);
+  // stores of a wave at the end of a tile, as far as a wait can count them
+  constexpr int ALL = RF * (PARTS ? CF : CF / 2);
+  constexpr int STORES = ALL < 63 - BEHIND ? ALL : 63 - BEHIND;
+  constexpr int XB = MT * FW_K, WB = WT * FW_K;              // bytes of a buffer
+  constexpr int HR = RF / 2, HC = CF / 2, Q = HR * HC;       // a quarter's
+  __shared__ __attribute__((aligned(16))) unsigned char lds[NR * XB + NW * WB];
+  const int tid = threadIdx.x, lane = tid & (WAVE_SIZE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE_SIZE);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int lc = lane & 15, lg = lane >> 4;
+  const int steps = (K + FW_K - 1) / FW_K, pairs = (steps + 1) / 2;
+  const int mt = (M + MT - 1) / MT, nt = (N + WT - 1) / WT;
+
+  // An XCD's tiles follow each other in blocks of 4 tiles of rows by all columns,
+  // rows first (of 8, 8192 rows of 28672 x 4096 take 3 % longer, others the same); one
+  // part of k behind the other.
+  const int xcd = blockIdx.x & 7, per = FW_CUS / 8, slot = blockIdx.x >> 3;
+  const int all = mt * nt * (PARTS ? splits : 1);
+  const int q = all / 8, r = all % 8;
+  const int count = xcd < r ? q + 1 : q;    // tiles of this XCD
+  const int start = xcd * q + min(xcd, r);
+  if (slot >= count) return;
+  const int rounds = (count - slot + per - 1) / per;
+  struct Place { int m0, n0, part, from, n; };  // n: pairs of steps, from step `from`
+  auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  auto place = [&](int round) {
+    int t = start + round * per + slot;
+    Place p{0, 0, 0, 0, pairs};
+    if constexpr (PARTS) {
+      p.part = t / (mt * nt);
+      t -= p.part * (mt * nt);
+      const int first = one((int)((long)pairs * p.part / splits));
+      p.from = first * 2;
+      p.n = one((int)((long)pairs * (p.part + 1) / splits)) - first;
+    }
+    const int g = t / (4 * nt), in = t % (4 * nt), high = min(4, mt - g * 4);
+    p.m0 = one((g * 4 + in % high) * MT);
+    p.n0 = one(in / high * WT);
+    return p;
+  };
+
+  // A wave's load i brings rows (i * 4 + wave) * 8 .. of 128 bytes to the LDS. Of two
+  // neighbouring tiles of 16 weight rows, rows 4 g .. are 8 neighbouring columns.
+  unsigned ox[RF], ow[CF];
+#pragma unroll
+  for (int i = 0; i < RF || i < CF; ++i) {
+    const int row = (i * 4 + wave) * 8 + lane / 8;
+    const int at = ((lane & 7) ^ ((row >> 1) & 7)) * 16;     // (the same for every i)
+    if (i < RF) ox[i] = (unsigned)row * (unsigned)K + at;
+    if (i < CF) {
+      const int b = row / 16 % CF, g = (row >> 2) & 3, j = row & 3;
+      const int col = row / (CF * 16) * (CF * 16) + b / 2 * 32 + g * 8 + (b & 1) * 4 + j;
+      ow[i] = (unsigned)col * (unsigned)K + at;
+    }
+  }
+  // of the last step of a row, where this lane's pieces (all its loads' are one) end
+  const int at = ((lane & 7) ^ ((wave * 4 + lane / 16) & 7)) * 16;
+  const unsigned behind = (steps - 1) * FW_K + at >= K ? 1u << 31 : 0u;
+  const int at0 = lc * FW_K + (lg ^ ((lc >> 1) & 7)) * 16;
+  const unsigned char* rl = lds + wm * (XB / 2) + at0;
+  const unsigned char* wl = lds + NR * XB + wn * (WB / 2) + at0;
+  const int other = at0 ^ 64;               // where a row's second piece is
+  const unsigned to =
+      lds_address(reinterpret_cast<const unsigned short*>(lds)) + wave * 8 * FW_K;
+
+  // The step that is loaded next: of the tile of round `lr`, with `left` steps to come;
+  // k0: its bytes from the start of a row. Each eighth of the columns begins an eighth
+  // of the row further on: weight rows lie a power of two apart, and workgroups at one
+  // place of theirs meet on a few memory channels.
+  auto turn = [&](const Place& p) {
+    return !PARTS && M <= 2048 ? one(p.n0 / WT * 8 / nt * steps / 8) : p.from;
+  };
+  int lr = 0, left = 0, past = 0;           // past: the step of zeros is in this tile
+  unsigned k0 = 0, out_of = 0;
+  i32x4 rx{}, rw{};
+  auto edge = [&]() { out_of = k0 + FW_K > (unsigned)K ? behind : 0u; };
+  auto point = [&]() {
+    if (lr < rounds) {
+      const Place p = place(lr);
+      left = 2 * p.n;
+      past = p.from + left > steps;
+      k0 = (unsigned)turn(p) * FW_K;
+      rx = wt_rsrc(x + (long)p.m0 * K, (unsigned)min(MT, M - p.m0) * (unsigned)K);
+      rw = wt_rsrc(w + (long)p.n0 * K, (unsigned)(N - p.n0) * (unsigned)K);
+    } else {
+      left = 2;
+      past = 0;
+      k0 = 0;
+      rx[2] = rw[2] = 0;
+    }
+  };
+  auto advance = [&]() {
+    k0 += FW_K;
+    if (!PARTS && k0 >= (unsigned)K) k0 = 0;
+    if (--left == 0) {
+      ++lr;
+      point();
+    } else if (left == 1 && past) {
+      rx[2] = rw[2] = 0;
+    }
+    edge();
+  };
+  auto load = [&](unsigned at, unsigned off, const i32x4& rs) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+                 "buffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(at), "v"(off | out_of), "s"(rs), "s"(k0)
+                 : "m0", "memory");
+  };
+  point();
+  edge();
+#pragma unroll
+  for (int s = 0; s < NR; ++s) {
+#pragma unroll
+    for (int i = 0; i < CF; ++i) load(to + NR * XB + s * WB + i * 4096, ow[i], rw);
+#pragma unroll
+    for (int i = 0; i < RF; ++i) load(to + s * XB + i * 4096, ox[i], rx);
+    advance();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NR - 1) * (RF + CF)) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  int bx = 0, bw = 0;                       // buffers of the step at hand
+
+  union Frag { u32x4 half[2]; i32x8 all; };
+  Frag fr[RF], fw[CF];
+  f32x4 acc[RF][CF];
+  // piece `h` of a row's 128 bytes, of tile i behind p
+  auto piece = [&](const unsigned char* p, int i, int h) {
+    return *reinterpret_cast<const u32x4*>(
+        (h ? p - at0 + other : p) + i * 16 * FW_K);
+  };
+#pragma unroll
+  for (int i = 0; i < HR; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) fr[i].half[h] = piece(rl, i, h);
+#pragma unroll
+  for (int i = 0; i < HC; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) fw[i].half[h] = piece(wl, i, h);
+
+  // One quarter: rows' half A, columns' half B. Into its gaps go the reads of `f`, the
+  // HR or HC operands from `from` on, and loads `first` .. to `dst`, one in every EVERY.
+  auto quarter = [&](auto a_, auto b_, auto n_, Frag* f, const unsigned char* from,
+                     auto first_, auto loads_, const i32x4& rs, unsigned dst,
+                     const unsigned* off) {
+    constexpr int A = decltype(a_)::value, B = decltype(b_)::value;
+    constexpr int READS = 2 * decltype(n_)::value;
+    constexpr int FIRST = decltype(first_)::value, LOADS = decltype(loads_)::value;
+    constexpr int EVERY = LOADS ? Q / LOADS : Q, AT = EVERY > 2 ? 2 : EVERY - 1;
+    // reads are done three quarters through
+    constexpr int WITHIN = Q * 3 / 4 > 0 ? Q * 3 / 4 : 1;
+    int done = 0;
+#ifdef __HIP_DEVICE_COMPILE__               // the host knows no register of 32 bytes
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      const int a = A * HR + i % HR, b = B * HC + i / HR, l = i / EVERY;
+      if (i % EVERY == AT && l < LOADS) {
+        asm volatile("s_add_u32 m0, %3, %4\n\t"
+                     "v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0\n\t"
+                     "buffer_load_dwordx4 %5, %6, %7 offen lds"
+                     : "+a"(acc[a][b])
+                     : "v"(fw[b].all), "v"(fr[a].all), "s"(dst), "n"((FIRST + l) * 4096),
+                       "v"(off[FIRST + l] | out_of), "s"(rs), "s"(k0)
+                     : "m0", "scc", "memory");
+      } else {
+        asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0"
+                     : "+a"(acc[a][b]) : "v"(fw[b].all), "v"(fr[a].all));
+      }
+      const int due = i + 1 >= WITHIN ? READS : ((i + 1) * READS + WITHIN - 1) / WITHIN;
+#pragma unroll
+      for (int j = 0; j < READS; ++j)
+        if (j >= done && j < due) {
+          __builtin_amdgcn_sched_barrier(0);
+          f[j / 2].half[j % 2] = piece(from, j / 2, j % 2);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      done = due;
+    }
+#endif
+  };
+  auto step = [&](auto odd_, bool after) {
+    constexpr int P = decltype(odd_)::value, L = 1 - P;
+    using LateR = wt_int<L>;
+    const int nx = bx == NR - 1 ? 0 : bx + 1;
+    const int nw = bw == NW - 1 ? 0 : bw + 1, over = bw == 0 ? NW - 1 : bw - 1;
+    const unsigned dw = to + NR * XB + over * WB, dx = to + bx * XB;
+    quarter(wt_int<P>{}, wt_int<0>{}, wt_int<HR>{}, fr + L * HR,
+            rl + bx * XB + L * HR * 16 * FW_K, wt_int<0>{}, wt_int<CF / 2>{}, rw, dw, ow);
+    quarter(LateR{}, wt_int<0>{}, wt_int<HC>{}, fw + HC, wl + bw * WB + HC * 16 * FW_K,
+            wt_int<CF / 2>{}, wt_int<CF / 2>{}, rw, dw, ow);
+    // the next step is there: BEHIND loads came after its own, and where those were
+    // asked for in the tile before, its stores
+    if (after)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BEHIND + STORES) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BEHIND) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    quarter(LateR{}, wt_int<1>{}, wt_int<HC>{}, fw, wl + nw * WB, wt_int<0>{},
+            wt_int<RF / 2>{}, rx, dx, ox);
+    quarter(wt_int<P>{}, wt_int<1>{}, wt_int<HR>{}, fr + L * HR,
+            rl + nx * XB + L * HR * 16 * FW_K, wt_int<RF / 2>{}, wt_int<RF / 2>{}, rx, dx,
+            ox);
+    advance();
+    bx = nx;
+    bw = nw;
+  };
+#pragma unroll 1
+  for (int round = 0; round < rounds; ++round) {
+#pragma unroll
+    for (int a = 0; a < RF; ++a)
+#pragma unroll
+      for (int b = 0; b < CF; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    asm volatile("s_nop 7" ::: "memory");
+    const Place p = place(round);
+#pragma unroll 1
+    for (int s = 0; s < p.n; ++s) {
+      step(wt_int<0>{}, round > 0 && 2 * s < NR - 1);
+      step(wt_int<1>{}, round > 0 && 2 * s + 1 < NR - 1);
+    }
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+
+    // acc[a][b][j]: row 4 lg + j of weight tile b, row lc of tile a
+    constexpr unsigned SIZE = PARTS ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+        (char*)out_ + (((long)p.part * M + p.m0) * N + p.n0) * SIZE, 0,
+        ((unsigned)min(MT, M - p.m0) - 1) * (unsigned)N * SIZE +
+            (unsigned)min(WT, N - p.n0) * SIZE,
+        0x00020000);
+    const int row0 = wm * (MT / 2) + lc;
+    unsigned row = (unsigned)row0 * (unsigned)N * SIZE;
+    asm volatile("" : "+v"(row));           // not a register for every row
+    float sx[RF];
+    if constexpr (!PARTS)
+#pragma unroll
+      for (int a = 0; a < RF; ++a) sx[a] = xs[min(p.m0 + row0 + a * 16, M - 1)];
+#pragma unroll
+    for (int b = 0; b < CF; b += 2) {
+      // columns and rows beyond the result are not stored; N is a multiple of 8
+      const int col = wn * (WT / 2) + b / 2 * 32 + lg * 8;
+      const bool in = p.n0 + col < N;
+      f32x4 sw[2];
+      u16x8 add{};
+      if constexpr (!PARTS) {
+        const int at = in ? p.n0 + col : 0;
+        sw[0] = *reinterpret_cast<const f32x4*>(ws + at);
+        sw[1] = *reinterpret_cast<const f32x4*>(ws + at + 4);
+        if (bias) add = *reinterpret_cast<const u16x8*>(bias + at);
+      }
+#pragma unroll
+      for (int a = 0; a < RF; ++a) {
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned off = in ? row + (unsigned)a * 16u * SIZE * (unsigned)N + col * SIZE
+                                : 0xffffff00u;
+        if constexpr (PARTS) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            u32x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              o[j] = __builtin_bit_cast(unsigned, wt_sum(acc[a][b + i][j]));
+            __builtin_amdgcn_raw_buffer_store_b128(o, ro, in ? off + i * 16 : off, 0, 0);
+          }
+        } else {
+          u32x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {     // two columns each
+            const f32x4 v = acc[a][b + j / 2], s = sw[j / 2];
+            const int e = j % 2 * 2;
+            o[j] = wt_pack(
+                __builtin_fmaf(wt_sum(v[e]), sx[a] * s[e], bf2f(add[2 * j])),
+                __builtin_fmaf(wt_sum(v[e + 1]), sx[a] * s[e + 1], bf2f(add[2 * j + 1])));
+          }
+          __builtin_amdgcn_raw_buffer_store_b128(o, ro, off, 0, 0);
+        }
+      }
+    }
+  }
+  // no load is left that would write to the LDS of a later workgroup
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+}  // namespace
+
+// rf, cf: a quarter of the tile in 16 rows and weight rows. Each part has a pair of
+// steps of k or more; offsets inside a tile's operands are 32 bits, 31 where rows end
+// within a step.
+void fp8_wide_launch(void* out, const void* x, const float* xs, const void* w,
+                     const float* ws, const void* bias, int M, int N, int K, int splits,
+                     int rf, int cf, int* err_unsupported, hipStream_t s) {
+  constexpr int MOST = 256;
+  const long far = K % FW_K ? 1l << 31 : 1l << 32;
+  *err_unsupported = K % 16 != 0 || K < FW_K || N % 8 != 0 ||
+                     ((long)N + MOST) * K >= far || (long)K * MOST >= far ||
+                     4l * N * (MOST + 1) >= (1l << 32) - 256 || splits < 1 ||
+                     ((K + FW_K - 1) / FW_K + 1) / 2 < splits || rf < 0 || rf > 9 || cf < 0 || cf > 9;
+  if (*err_unsupported || M == 0 || N == 0) return;
+  switch ((splits > 1) * 100 + rf * 10 + cf) {
+#define WIDE(PARTS, RF, CF)                                                            \
+    case PARTS * 100 + RF * 10 + CF:                                                   \
+      hipLaunchKernelGGL((fp8_wide_kernel<PARTS != 0, RF, CF>), dim3(FW_CUS),          \
+                         dim3(256), 0, s, out, (const unsigned char*)x, xs,            \
+                         (const unsigned char*)w, ws, (const unsigned short*)bias, M, N, \
+                         K, splits);                                                   \
+      break
+    WIDE(0, 8, 8); WIDE(0, 8, 6); WIDE(0, 8, 4); WIDE(0, 6, 8); WIDE(0, 6, 6);
+    WIDE(0, 4, 8); WIDE(0, 4, 6); WIDE(0, 4, 4); WIDE(0, 4, 2);
+    WIDE(1, 8, 8); WIDE(1, 8, 6); WIDE(1, 8, 4); WIDE(1, 6, 8); WIDE(1, 6, 6);
+    WIDE(1, 4, 8); WIDE(1, 4, 6); WIDE(1, 4, 4); WIDE(1, 4, 2);
+#undef WIDE
+    default: *err_unsupported = 1;
+  }
+}
