@@ -25,7 +25,7 @@ HEADERS = ["common.h", "wide_tiles.h", "pinned_words.h"]
 # that serves only such a model compiles these few files and nothing else
 LATENT_SO_PATH = PKG_DIR / "_hip_latent.so"
 SMALL_HEADERS = ["common.h", "short_conv_binding.h", "pinned_words.h",
-                 "wide_tiles.h"]
+                 "wide_tiles.h", "lora.h"]
 LATENT_SOURCES = ["resid32.hip", "latent_attn.hip", "grouped_ff.hip",
                   "latent_bindings.cpp"]
 

@@ -6,6 +6,8 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include "lora.h"
+
 int fp8_rows_most();
 void fp8_rows_launch(int, void*, float*, void*, void*, const void*, long, const void*, const void*, float, int, int, hipStream_t);
 void fp8_rows_gemm_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, hipStream_t);
@@ -15,7 +17,8 @@ void fp8_tile_launch(void*, const void*, const float*, const void*, const float*
 void fp8_join_launch(void*, const void*, const float*, const float*, const void*, int, int, int, hipStream_t);
 void fp8_wide_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, int, int*, hipStream_t);
 int lora_most_rank();
-void lora_launch(void*, long, float*, const void*, long, const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, const int*, int, int, int, hipStream_t);
+LoraPlan lora_plan(bool, bool, int);
+void lora_launch(void*, long, float*, const void*, long, const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, const int*, int, LoraPlan, int, int, hipStream_t);
 
 #define HIP_CHECK_LAST()                                                     \
   do {                                                                       \
@@ -183,20 +186,30 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
   TORCH_CHECK(starts.size(0) == S + 1 && ranks.size(0) == S,
               "lora_add: S + 1 starts and S ranks");
   TORCH_CHECK(T <= rows && rows < 1l << 31 && S < 1l << 24 && N < 1l << 31 && K < 1l << 31 &&
-              (N + 255) / 256 + P <= 65535, "lora_add: sizes");
+              (T + S) / 16 <= 65535 * 8, "lora_add: sizes");
   if (T == 0 || S == 0) return;
   const at::DeviceGuard guard(x.device());
-  // tiles of 64 rows where a slot has half of one on average, else of 16. k is cut until
-  // there are two workgroups a CU, each wave having a unit of 64 k of its own at least
-  const int tt = T >= 32 * std::min(S, T) ? 4 : 1;
-  const long tiles = std::min(T, (T + std::min(S, T) * (16 * tt - 1)) / (16 * tt));
-  const long groups = (P * ((R + 15) / 16) + tt - 1) / tt;
-  const long splits = std::max(1l, std::min({512 / (tiles * groups), (K + 255) / 256, 16l}));
+  // 16 rows a tile below 32 rows a slot on average, 64 below 128, else 128
+  const long used = std::min(S, T), groups = P * ((R + 15) / 16);
+  const LoraPlan plan = lora_plan(T < 32 * used, T >= 128 * used, (int)groups);
+  // k is cut until the workgroups fill the CUs: of few rows each wave has four units of
+  // 64 k then; of many at least four steps are left, and up to five parts, which the
+  // second launch reads again for every 512 columns (8192 rows of 4096 x 4096 at rank 64
+  // in 1, 3 and 7 parts: 38 + 47, 22 + 55 and 23 + 62 us)
+  const long tiles = (long)lora_tiles(T, S, 16 * plan.mt) * ((groups + plan.nt - 1) / plan.nt);
+  const long units = (K + 63) / 64;
+  const long splits = std::max(1l, plan.mt == 1
+      ? std::min((units + 15) / 16, 4096 / tiles)
+      : std::min({units / 4, 256 * plan.held / tiles, 5l}));
+  // 256 columns of 16 or 32 rows at a time, more in turn where that leaves 1024 workgroups
+  const bool few = plan.mt == 1;
+  const long turns = std::max(1l, std::min(few ? 4l : 2l, lora_tiles(T, S, few ? 16 : 32) *
+                                                              ((N + 255) / 256) / 1024));
   Tensor h = at::empty({splits, T, P * R}, x.options().dtype(at::kFloat));
   lora_launch(out.data_ptr(), os, h.data_ptr<float>(), x.data_ptr(), xs, a.data_ptr(),
               b.data_ptr(), order.data_ptr<int>(), starts.data_ptr<int>(),
               ranks.data_ptr<int>(), (int)rows, (int)T, (int)S, (int)N, (int)K, (int)P, e,
-              (int)R, tt, (int)splits, cur_stream(x));
+              (int)R, plan, (int)splits, (int)turns, cur_stream(x));
   HIP_CHECK_LAST();
 }
 

@@ -54,13 +54,7 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
   auto block = [&](int b) { return b + rot < nb ? b + rot : b + rot - nb; };
   auto piece = [&](const unsigned char* p, int b, int c) {
     const int k = b * FR_K + c * 64 + lg * 16;
-    if constexpr (TAIL) {
-      u32x4 v = *reinterpret_cast<const u32x4*>(p + (k < K ? k : 0));
-      if (k >= K) v = u32x4{0, 0, 0, 0};
-      return v;
-    } else {
-      return *reinterpret_cast<const u32x4*>(p + k);
-    }
+    return *reinterpret_cast<const u32x4*>(p + (TAIL && k >= K ? 0 : k));
   };
   u32x4 wc[NTW][4], wn[NTW][4], xc[MT][4], xn[MT][4];
   auto fetch = [&](u32x4 (&wv)[NTW][4], u32x4 (&xv)[MT][4], int b) {
@@ -80,7 +74,19 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
 #pragma unroll
     for (int t = 0; t < NTW; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto products = [&] {
+  // pieces behind the end of the rows came from their start: cleared here, since a
+  // clearing where they are asked for would wait for them
+  auto products = [&](int b) {
+    if constexpr (TAIL)
+      if (b == nb - 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (b * FR_K + c * 64 + lg * 16 >= K) {
+#pragma unroll
+            for (int t = 0; t < NTW; ++t) wc[t][c] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xc[m][c] = u32x4{0, 0, 0, 0};
+          }
 #pragma unroll
     for (int c = 0; c < 4; c += 2)
 #pragma unroll
@@ -93,7 +99,7 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
   int i = wave;
   for (; i + FR_WAVES < nb; i += FR_WAVES) {
     fetch(wn, xn, block(i + FR_WAVES));
-    products();
+    products(block(i));
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -102,7 +108,7 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
       for (int m = 0; m < MT; ++m) xc[m][c] = xn[m][c];
     }
   }
-  if (i < nb) products();
+  if (i < nb) products(block(i));
 
   // D[row = lg * 4 + r][column = lc] per tile
 #pragma unroll

@@ -3,16 +3,20 @@
 // for every row m whose request has adapter s; p: the part (q, k, v; gate, up) that
 // column n belongs to; j below the adapter's own rank, what lies behind it in a and b
 // is not used. The rows come in an order in which those of one adapter are neighbours
-// (order, starts), so a tile of 16 TT rows has one adapter and the matrix unit's
+// (order, starts), so a tile of rows has one adapter and the matrix unit's
 // 16 x 16 x 32 products serve decode steps and prompts alike.
 //
-// Two launches. The first multiplies by a, with k cut over the grid and over a
-// workgroup's four waves: a wave's rows and weights go straight to its registers,
-// each read once. Its fp32 sums (h, in `splits` parts) are added up by the second,
+// Two launches. The first multiplies by a, with k cut over the grid where there are few
+// tiles. Its fp32 sums (h, in `splits` parts) are added up by the second,
 // which holds them as two bf16 parts (the value and what that rounded away, 16 bits of
 // it in all): one would cost h the 2^-9 that the rest of the sum does not lose. Both
-// are bound by memory: x and a, then b and out.
-#include "common.h"
+// are bound by memory: x and a, then b and out. us, first and second: one row of 4096 k
+// and 6144 columns in three parts, rank 16, 4.2 and 4.5; 64 rows of 28 adapters, 28672
+// columns in two parts, ranks 1 to 64 of 64, 9 and 27 (of rank 16 in 16, 6 and 9); 2039
+// rows of 8 runs, 6144 columns, rank 32, 15 and 17; 8192 rows, 4096 columns, rank 64, 24
+// and 56, rank 16, 22 and 33; 28672 columns, rank 16, 22 and 200, where adding a number to
+// as many takes 158.
+#include "lora.h"
 
 namespace {
 
@@ -62,115 +66,207 @@ DEVICE_INLINE Place find_tile(int tile, const int* starts, const int* ranks, int
   return Place{0, 0, 0, 0};
 }
 
-// h, [splits, T, C] by place in the order. Tiles of 16 TT rows; CT tiles of 16 of the
-// C = P R columns, of which an adapter has the ceil(rank / 16) first of each part.
-template <int TT, int CT>
+// h, [splits, T, C] by place in the order, for few rows an adapter: a workgroup has 16
+// rows and one of the tiles of 16 of the C = P R columns, of which an adapter has the
+// ceil(rank / 16) first of each part. The four waves take the units of 64 k in turn,
+// four of each at a time, straight to the registers, and meet in the LDS.
 __global__ __launch_bounds__(256) void lora_down_kernel(
     float* __restrict__ h, const unsigned short* __restrict__ x, long xs,
     const unsigned short* __restrict__ a, const int* __restrict__ order,
     const int* __restrict__ starts, const int* __restrict__ ranks, int rows, int T, int S,
     int K, int P, int R) {
-  constexpr int ROWS = 16 * TT, U = 64;
-  __shared__ f32x4 red[4 * TT * CT * WAVE_SIZE];
+  constexpr int U = 64, UN = 4;
+  __shared__ f32x4 red[4 * WAVE_SIZE];
+  const Place p = find_tile<16>(blockIdx.x, starts, ranks, S, T, R);
+  const int each = (p.rank + 15) / 16;       // tiles of a part
+  if (p.count == 0 || (int)blockIdx.y >= P * each) return;
+  const int tid = threadIdx.x, lane = tid & (WAVE_SIZE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE_SIZE);
+  const int lc = lane & 15, lg = lane >> 4;
+  const int C = P * R, part = blockIdx.y / each, j0 = (blockIdx.y - part * each) * 16;
+
+  const int row = order[p.first + min(lc, p.count - 1)];
+  const unsigned short* xp = x + min(max(row, 0), rows - 1) * xs;
+  const unsigned short* ap =
+      a + ((long)p.slot * C + part * R + min(j0 + lc, p.rank - 1)) * K;
+  const int units = (K + U - 1) / U, splits = gridDim.z;
+  const int from = (int)((long)units * blockIdx.z / splits);
+  const int n = (int)((long)units * (blockIdx.z + 1) / splits) - from;
+  f32x4 acc{0.f, 0.f, 0.f, 0.f};
+  for (int u = wave; u < n; u += 4 * UN) {
+    // a lane's pieces of a unit: 8 k for each of two products. Pieces behind the end of
+    // the rows come from their start and are cleared where they are used: here that
+    // would wait for them.
+    auto place = [&](int m, int i) {
+      return (from + min(u + 4 * m, n - 1)) * U + i * 32 + lg * 8;
+    };
+    u32x4 fx[UN][2], fa[UN][2];
+#pragma unroll
+    for (int m = 0; m < UN; ++m)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = place(m, i) < K ? place(m, i) : 0;
+        fa[m][i] = *reinterpret_cast<const u32x4*>(ap + k);
+        fx[m][i] = *reinterpret_cast<const u32x4*>(xp + k);
+      }
+#pragma unroll
+    for (int m = 0; m < UN; ++m) {
+      if (u + 4 * m >= n) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (place(m, i) >= K) fa[m][i] = fx[m][i] = u32x4{0, 0, 0, 0};
+        acc = multiply(fa[m][i], fx[m][i], acc);
+      }
+    }
+  }
+  red[tid] = acc;
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) acc += red[w * WAVE_SIZE + lane];
+  // D[column = lg * 4 + r][row = lc]
+  const int j = j0 + lg * 4;
+  if (lc < p.count && j < R)
+    *reinterpret_cast<f32x4*>(h + ((long)blockIdx.z * T + p.first + lc) * C + part * R + j) =
+        acc;
+}
+
+// The same of prompts: tiles of 16 MT rows, and 16 NT of an adapter's columns, a step of
+// 64 k of both through a ring of S buffers in the LDS, filled S - 1 steps ahead (to the
+// registers, a wave with rows and columns of its own k, 8192 rows of 4096 k at 64 columns
+// take 33 us where these take DOWN_US). Rows of 128 bytes, 16-byte piece c of row r at
+// c ^ (r / 2 % 8), which 16 rows read without conflict. Each of the four waves has MT / 4
+// tiles of rows and all columns, so there is nothing to add up in the workgroup.
+__device__ const u32x4 lora_zeros = {0, 0, 0, 0};
+
+template <int MT, int NT, int S_>
+__global__ __launch_bounds__(256) void lora_down_tile_kernel(
+    float* __restrict__ h, const unsigned short* __restrict__ x, long xs,
+    const unsigned short* __restrict__ a, const int* __restrict__ order,
+    const int* __restrict__ starts, const int* __restrict__ ranks, int rows, int T, int S,
+    int K, int P, int R) {
+  constexpr int ROWS = 16 * MT, U = 64, BUF = (ROWS + 16 * NT) * U, RT = MT / 4;
+  constexpr int L = (MT + NT) / 2;           // loads of a wave in a step
+  static_assert(MT % 4 == 0 && NT % 2 == 0 && S_ >= 2 && S_ <= 4 && 2 * L <= 63, "waits");
+  __shared__ __attribute__((aligned(16))) unsigned short lds[S_ * BUF];
   const Place p = find_tile<ROWS>(blockIdx.x, starts, ranks, S, T, R);
   const int each = (p.rank + 15) / 16;       // tiles of a part
-  const int c0 = blockIdx.y * CT;
-  if (p.count == 0 || c0 >= P * each) return;
+  const int c0 = blockIdx.y * NT, tiles = P * each;
+  if (p.count == 0 || c0 >= tiles) return;
   const int tid = threadIdx.x, lane = tid & (WAVE_SIZE - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE_SIZE);
   const int lc = lane & 15, lg = lane >> 4;
   const int C = P * R;
 
-  const unsigned short* xp[TT];
+  // a wave's load fills 8 rows; wave w takes every fourth of them
+  const int at = ((lane & 7) ^ ((wave * 4 + lane / 16) & 7)) * 8;
+  const unsigned short* from[L];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    const int row = order[p.first + min(t * 16 + lc, p.count - 1)];
-    xp[t] = x + min(max(row, 0), rows - 1) * xs + lg * 16;
-  }
-  const unsigned short* ap[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int i = min(c0 + c, P * each - 1);
-    const int j = min(i % each * 16 + lc, p.rank - 1);
-    ap[c] = a + ((long)p.slot * C + i / each * R + j) * K + lg * 16;
+  for (int i = 0; i < L; ++i) {
+    const int r = (i * 4 + wave) * 8 + lane / 8;
+    if (i < MT / 2) {
+      const int row = order[p.first + min(r, p.count - 1)];
+      from[i] = x + min(max(row, 0), rows - 1) * xs;
+    } else {
+      const int c = min(c0 + (r - ROWS) / 16, tiles - 1), part = c / each;
+      const int j = min((c - part * each) * 16 + r % 16, p.rank - 1);
+      from[i] = a + ((long)p.slot * C + part * R + j) * K;
+    }
   }
   const int units = (K + U - 1) / U, splits = gridDim.z;
-  const int from = (int)((long)units * blockIdx.z / splits);
-  const int to = (int)((long)units * (blockIdx.z + 1) / splits);
-  f32x4 acc[TT][CT];
+  const int first = (int)((long)units * blockIdx.z / splits);
+  const int n = (int)((long)units * (blockIdx.z + 1) / splits) - first;
+  // tiles begin at places of their own: rows lie a power of two apart
+  const int rot = blockIdx.x * 7 % n;
+  auto stage = [&](int i) {
+    const int k0 = (first + (i + rot < n ? i + rot : i + rot - n)) * U;
+    unsigned short* to = lds + i % S_ * BUF + wave * 8 * U;
+    const bool past = k0 + at >= K;
 #pragma unroll
-  for (int t = 0; t < TT; ++t)
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  // a lane's 16 neighbours of a unit of 64 k, 8 for each of two products
-  for (int u = from + wave; u < to; u += 4) {
-    const int k = u * U;
-    u32x4 fx[TT][2], fa[CT][2];
-    auto piece = [&](const unsigned short* q, int i) {
-      const bool in = k + lg * 16 + i * 8 < K;
-      u32x4 v = *reinterpret_cast<const u32x4*>(in ? q + k + i * 8 : q - lg * 16);
-      if (!in) v = u32x4{0, 0, 0, 0};
-      return v;
-    };
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int t = 0; t < TT; ++t) fx[t][i] = piece(xp[t], i);
-#pragma unroll
-      for (int c = 0; c < CT; ++c) fa[c][i] = piece(ap[c], i);
+    for (int j = 0; j < L; ++j) {
+      const unsigned short* v = from[j] + k0 + at;
+      if (k0 + U > K) v = past ? reinterpret_cast<const unsigned short*>(&lora_zeros) : v;
+      load_to_lds(v, to + j * 32 * U);
     }
+  };
+  f32x4 acc[RT][NT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
+    for (int c = 0; c < NT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-          acc[t][c] = multiply(fa[c][i], fx[t][i], acc[t][c]);
+  for (int i = 0; i < S_ - 1; ++i)
+    if (i < n) stage(i);
+  const int a0 = lc * U + (lg ^ ((lc >> 1) & 7)) * 8;
+  for (int i = 0; i < n; ++i) {
+    const int ahead = min(S_ - 2, n - 1 - i);
+    if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * L) : "memory");
+    else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(L) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (i + S_ - 1 < n) stage(i + S_ - 1);
+    const unsigned short* xl = lds + i % S_ * BUF + wave * RT * 16 * U;
+    const unsigned short* al = lds + i % S_ * BUF + ROWS * U;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int o = a0 ^ (q * 32);
+      u32x4 fx[RT], fa[NT];
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+        fa[c] = *reinterpret_cast<const u32x4*>(al + c * 16 * U + o);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        fx[t] = *reinterpret_cast<const u32x4*>(xl + t * 16 * U + o);
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t][c] = multiply(fa[c], fx[t], acc[t][c]);
+    }
   }
-#pragma unroll
-  for (int t = 0; t < TT; ++t)
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-      red[((wave * TT + t) * CT + c) * WAVE_SIZE + lane] = acc[t][c];
-  __syncthreads();
   // D[column = lg * 4 + r][row = lc] per tile
-  for (int i = wave; i < TT * CT; i += 4) {
-    f32x4 v = red[i * WAVE_SIZE + lane];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) v += red[(w * TT * CT + i) * WAVE_SIZE + lane];
-    const int row = i / CT * 16 + lc, c = c0 + i % CT;
-    const int j = c % each * 16 + lg * 4;
-    if (row < p.count && c < P * each && j < R)
-      *reinterpret_cast<f32x4*>(h + ((long)blockIdx.z * T + p.first + row) * C +
-                                c / each * R + j) = v;
+  for (int c = 0; c < NT; ++c) {
+    if (c0 + c >= tiles) break;
+    const int part = (c0 + c) / each, j = (c0 + c - part * each) * 16 + lg * 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = (wave * RT + t) * 16 + lc;
+      if (row < p.count && j < R)
+        *reinterpret_cast<f32x4*>(h + ((long)blockIdx.z * T + p.first + row) * C +
+                                  part * R + j) = acc[t][c];
+    }
   }
 }
 
 struct Ends { int n, end[4]; };
 
-// out += h b^T. A workgroup has 16 TT rows and 256 columns of one part, its waves 64
-// each: four tiles of 16 weight rows, dealt so that a lane ends with 16 neighbours of
-// a row. KT: 32 k of the rank at a time that the registers hold (32 KT >= rank).
+// out += h b^T. A workgroup has 16 TT rows and `turns` times 256 columns of one part,
+// its waves 64 of them each, so that what is read and written of a row at about one time
+// is 512 neighbouring bytes and more (of 128 rows and 64 columns a workgroup 28672 columns
+// take 236 us for 200): four tiles of 16 weight rows, dealt so that a lane ends
+// with twice 8 neighbours of a row and four lanes with 64 bytes of it. What a turn reads
+// of b and out is asked for before the turn before ends, the first turn's before h. KT:
+// 32 k of the rank at a time that the registers hold (32 KT >= rank).
 template <int TT, int KT>
 __global__ __launch_bounds__(256) void lora_up_kernel(
     unsigned short* __restrict__ out, long os, const float* __restrict__ h, int splits,
     const unsigned short* __restrict__ b, const int* __restrict__ order,
     const int* __restrict__ starts, const int* __restrict__ ranks, int rows, int T, int S,
-    int N, int R, Ends ends) {
+    int N, int R, int turns, Ends ends) {
   constexpr int ROWS = 16 * TT, LD = 32 * KT + 8;
   __shared__ __attribute__((aligned(16))) unsigned short part[2][ROWS * LD];
-  const Place p = find_tile<ROWS>(blockIdx.x, starts, ranks, S, T, R);
+  const Place p = find_tile<ROWS>(blockIdx.y, starts, ranks, S, T, R);
   if (p.count == 0 || p.rank == 0) return;
   const int tid = threadIdx.x, lane = tid & (WAVE_SIZE - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE_SIZE);
   const int lc = lane & 15, lg = lane >> 4;
-  const int C = ends.n * R;
+  const int C = ends.n * R, wide = 256 * turns;
 
-  int block = blockIdx.y, which = 0, low = 0, high = ends.end[0];
+  int block = blockIdx.x, which = 0, low = 0, high = ends.end[0];
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    const int blocks = (high - low + 255) / 256;
+    const int blocks = (high - low + wide - 1) / wide;
     if (i < ends.n - 1 && which == i && block >= blocks) {
       block -= blocks;
       which = i + 1;
@@ -178,80 +274,105 @@ __global__ __launch_bounds__(256) void lora_up_kernel(
       high = ends.end[i + 1];
     }
   }
-  const int n0 = low + block * 256 + wave * 64;
+  const int last = min(low + (block + 1) * wide, high);
+  int n0 = low + block * wide + wave * 64;
 
+  int at[TT];                                // rows of out, below 0 where there is none
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    const int i = t * 16 + lc;
+    const int row = i < p.count ? order[p.first + i] : -1;
+    at[t] = row < rows ? row : -1;
+  }
+  u32x4 fb[KT][4];
+  u16x8 old[TT][2];
+  // row i of tile c is column c / 2 * 32 + i / 4 * 8 + c % 2 * 4 + i % 4
+  auto weights = [&](int n) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = k * 32 + lg * 8;
+        const int col = min(n + c / 2 * 32 + (lc >> 2) * 8 + c % 2 * 4 + (lc & 3), high - 1);
+        fb[k][c] = *reinterpret_cast<const u32x4*>(
+            b + ((long)p.slot * N + col) * R + (j < p.rank ? j : 0));
+      }
+  };
+  auto before = [&](int n) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int col = n + g * 32 + lg * 8;
+        old[t][g] = *reinterpret_cast<const u16x8*>(
+            out + (at[t] < 0 ? 0 : at[t]) * os + (col < high ? col : low));
+      }
+  };
+  weights(min(n0, last - 1));
+  before(min(n0, last - 1));
   for (int i = tid; i < ROWS * 8 * KT; i += 256) {
     const int row = i / (8 * KT), j = i % (8 * KT) * 4;
     f32x4 v{0.f, 0.f, 0.f, 0.f};
     if (row < p.count && j < p.rank) {
-      const float* at = h + (long)(p.first + row) * C + which * R + j;
+      const float* from = h + (long)(p.first + row) * C + which * R + j;
+#pragma unroll 4
       for (int s = 0; s < splits; ++s)
-        v += *reinterpret_cast<const f32x4*>(at + (long)s * T * C);
+        v += *reinterpret_cast<const f32x4*>(from + (long)s * T * C);
     }
     u16x4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (j + e >= p.rank) v[e] = 0.f;
       hi[e] = f2bf(v[e]);
-      lo[e] = f2bf(v[e] - bf2f(hi[e]));
+      // (an infinity leaves none)
+      lo[e] = __builtin_isinf(v[e]) ? (unsigned short)0 : f2bf(v[e] - bf2f(hi[e]));
     }
     *reinterpret_cast<u16x4*>(&part[0][row * LD + j]) = hi;
     *reinterpret_cast<u16x4*>(&part[1][row * LD + j]) = lo;
   }
   __syncthreads();
-  if (n0 >= high) return;
 
-  f32x4 acc[TT][4];
+  for (; n0 < last; n0 += 256) {
+    f32x4 acc[TT][4];
 #pragma unroll
-  for (int t = 0; t < TT; ++t)
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < 4; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < KT; ++k) {
-    if (k * 32 >= p.rank) break;
-    const int j = k * 32 + lg * 8, left = p.rank - j;
-    u32x4 fb[4];
+    for (int k = 0; k < KT; ++k) {
+      if (k * 32 >= p.rank) break;
+      const int j = k * 32 + lg * 8, left = p.rank - j;
+      if (left < 8)                          // what lies behind the rank may be anything
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      // row i of tile c is column i / 4 * 16 + c * 4 + i % 4
-      const int col = min(n0 + (lc >> 2) * 16 + c * 4 + (lc & 3), high - 1);
-      fb[c] = u32x4{0, 0, 0, 0};
-      if (left > 0) {
-        fb[c] = *reinterpret_cast<const u32x4*>(b + ((long)p.slot * N + col) * R + j);
-        if (left < 8)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            fb[c][e] &= 2 * e + 1 < left ? ~0u : 2 * e < left ? 0xffffu : 0u;
+            fb[k][c][e] &= 2 * e + 1 < left ? ~0u : 2 * e < left ? 0xffffu : 0u;
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(&part[0][(t * 16 + lc) * LD + j]);
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(&part[1][(t * 16 + lc) * LD + j]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          acc[t][c] = multiply(fb[k][c], lo, multiply(fb[k][c], hi, acc[t][c]));
       }
     }
+    const bool more = n0 + 256 < last;
+    if (more) weights(n0 + 256);
+    // acc[t][c][r]: row t * 16 + lc, column c / 2 * 32 + lg * 8 + c % 2 * 4 + r; ends are
+    // multiples of 8
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const u32x4 hi = *reinterpret_cast<const u32x4*>(&part[0][(t * 16 + lc) * LD + j]);
-      const u32x4 lo = *reinterpret_cast<const u32x4*>(&part[1][(t * 16 + lc) * LD + j]);
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        acc[t][c] = multiply(fb[c], lo, multiply(fb[c], hi, acc[t][c]));
-    }
-  }
-  // acc[t][c][r]: row t * 16 + lc, column lg * 16 + c * 4 + r; ends are multiples of 8
+      for (int g = 0; g < 2; ++g) {
+        const int col = n0 + g * 32 + lg * 8;
+        u16x8 v;
 #pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    const int i = t * 16 + lc;
-    if (i >= p.count) continue;
-    const int row = order[p.first + i];
-    if (row < 0 || row >= rows) continue;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int col = n0 + lg * 16 + g * 8;
-      if (col >= high) continue;
-      u16x8* at = reinterpret_cast<u16x8*>(out + row * os + col);
-      const u16x8 old = *at;
-      u16x8 v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = f2bf(bf2f(old[e]) + acc[t][g * 2 + e / 4][e % 4]);
-      *at = v;
-    }
+        for (int e = 0; e < 8; ++e)
+          v[e] = f2bf(bf2f(old[t][g][e]) + acc[t][g * 2 + e / 4][e % 4]);
+        if (at[t] >= 0 && col < high) *reinterpret_cast<u16x8*>(out + at[t] * os + col) = v;
+      }
+    if (more) before(n0 + 256);
   }
 }
 
@@ -259,43 +380,60 @@ __global__ __launch_bounds__(256) void lora_up_kernel(
 
 int lora_most_rank() { return 256; }
 
+// The tile's rows and columns of the first launch in 16, workgroups of it a CU holds.
+// few: 16 rows, one tile of columns; else by the tiles of columns that there are.
+LoraPlan lora_plan(bool few, bool many, int groups) {
+  if (few) return {1, 1, 8};
+  const int nt = groups <= 2 ? 2 : groups <= 4 ? 4 : groups <= 8 ? 8 : 12;
+  return {many ? 8 : 4, nt, nt <= 4 ? 2 : 1};
+}
+
 // rows: of x and out; T: entries of the order. K, R and the ends are multiples of 8.
-// tt (1 or 4): tiles of 16 rows a workgroup.
+// splits: parts of k of h; turns: of 256 columns a workgroup of the second launch.
 void lora_launch(void* out, long os, float* h, const void* x, long xs, const void* a,
                  const void* b, const int* order, const int* starts, const int* ranks,
                  int rows, int T, int S, int N, int K, int P, const int* ends, int R,
-                 int tt, int splits, hipStream_t s) {
-  const int each = 16 * tt;
-  // of S slots at most T have rows
-  const int tiles = (int)min((long)T, (T + (long)min(S, T) * (each - 1)) / each);
+                 LoraPlan plan, int splits, int turns, hipStream_t s) {
   const int groups = P * ((R + 15) / 16);
-  auto down = [&](auto kernel, int ct) {
-    hipLaunchKernelGGL(kernel, dim3(tiles, (groups + ct - 1) / ct, splits), dim3(256), 0,
-                       s, h, (const unsigned short*)x, xs, (const unsigned short*)a,
-                       order, starts, ranks, rows, T, S, K, P, R);
+  auto down = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel,
+                       dim3(lora_tiles(T, S, 16 * plan.mt),
+                            (groups + plan.nt - 1) / plan.nt, splits),
+                       dim3(256), 0, s, h, (const unsigned short*)x, xs,
+                       (const unsigned short*)a, order, starts, ranks, rows, T, S, K, P, R);
   };
-  if (tt == 1) down(lora_down_kernel<1, 1>, 1);
-  else down(lora_down_kernel<4, 4>, 4);
+  switch (plan.mt * 100 + plan.nt) {
+    case 101: down(lora_down_kernel); break;
+    case 402: down(lora_down_tile_kernel<4, 2, 4>); break;
+    case 404: down(lora_down_tile_kernel<4, 4, 4>); break;
+    case 408: down(lora_down_tile_kernel<4, 8, 4>); break;
+    case 412: down(lora_down_tile_kernel<4, 12, 4>); break;
+    case 802: down(lora_down_tile_kernel<8, 2, 4>); break;
+    case 804: down(lora_down_tile_kernel<8, 4, 3>); break;
+    case 808: down(lora_down_tile_kernel<8, 8, 4>); break;
+    case 812: down(lora_down_tile_kernel<8, 12, 4>); break;
+  }
   Ends e{P, {0, 0, 0, 0}};
+  const int wide = 256 * turns;
   int blocks = 0;
   for (int i = 0; i < P; ++i) {
     e.end[i] = ends[i];
-    blocks += (ends[i] - (i ? ends[i - 1] : 0) + 255) / 256;
+    blocks += (ends[i] - (i ? ends[i - 1] : 0) + wide - 1) / wide;
   }
-  auto up = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(tiles, blocks), dim3(256), 0, s,
+  auto up = [&](auto kernel, int tt) {
+    hipLaunchKernelGGL(kernel, dim3(blocks, lora_tiles(T, S, 16 * tt)), dim3(256), 0, s,
                        (unsigned short*)out, os, h, splits, (const unsigned short*)b,
-                       order, starts, ranks, rows, T, S, N, R, e);
+                       order, starts, ranks, rows, T, S, N, R, turns, e);
   };
-  if (tt == 1) {
-    if (R <= 32) up(lora_up_kernel<1, 1>);
-    else if (R <= 64) up(lora_up_kernel<1, 2>);
-    else if (R <= 128) up(lora_up_kernel<1, 4>);
-    else up(lora_up_kernel<1, 8>);
+  if (plan.mt == 1) {
+    if (R <= 32) up(lora_up_kernel<1, 1>, 1);
+    else if (R <= 64) up(lora_up_kernel<1, 2>, 1);
+    else if (R <= 128) up(lora_up_kernel<1, 4>, 1);
+    else up(lora_up_kernel<1, 8>, 1);
   } else {
-    if (R <= 32) up(lora_up_kernel<4, 1>);
-    else if (R <= 64) up(lora_up_kernel<4, 2>);
-    else if (R <= 128) up(lora_up_kernel<4, 4>);
-    else up(lora_up_kernel<4, 8>);
+    if (R <= 32) up(lora_up_kernel<2, 1>, 2);
+    else if (R <= 64) up(lora_up_kernel<4, 2>, 4);
+    else if (R <= 128) up(lora_up_kernel<2, 4>, 2);
+    else up(lora_up_kernel<2, 8>, 2);
   }
 }
