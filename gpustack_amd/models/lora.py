@@ -7,10 +7,12 @@ adapters, which gpustack surfaces as per-LoRA child model routes
 merge_lora) remains the zero-overhead path for a single adapter; this
 module serves MANY adapters concurrently: each batch row carries an
 adapter slot, and every target projection adds its low-rank delta
-  out[rows] += (x[rows] @ A^T) @ B^T * (alpha / r)
-for the rows of each active adapter. Deltas ride hipBLASLt GEMMs shaped
-[t, r] x [r, out] — skinny but tiny next to the base GEMM at realistic
-rank (r <= 64), so decode stays HBM-bound on the base weights.
+  out[t] += (x[t] @ A^T) @ B^T * (alpha / r)
+of the row's own adapter. The adapters' matrices of one fused projection
+(q|k|v, o, gate|up, down) lie stacked in one bank, so that ops.lora_add adds
+the deltas of all adapters of a batch in two launches, whichever rows have
+which; what that kernel does not take (other types than bf16 on the GPU, ranks
+over 256) goes adapter by adapter through library products.
 
 TP sharding matches the base layout: column-parallel targets (q/k/v,
 gate/up) shard B's output rows per rank; row-parallel targets (o, down)
@@ -25,9 +27,10 @@ from pathlib import Path
 
 import torch
 
+from .. import ops
+
 logger = logging.getLogger(__name__)
 
-# projection key -> (parent module, fused buffer, slice resolver)
 _ATTN_KEYS = ("q_proj", "k_proj", "v_proj", "o_proj")
 _MLP_KEYS = ("gate_proj", "up_proj", "down_proj")
 
@@ -121,8 +124,45 @@ class LoraAdapter:
         return cls(name, mods, rank_seen)
 
 
+class LoraGroup:
+    """The adapters' matrices of one fused projection: a [S, P R, K] and
+    b [S, N, R], part p (of columns up to ends[p]) reading rows p R .. of a;
+    zeros where an adapter has no such projection or a lower rank."""
+
+    def __init__(self, projs: list[tuple[str, int]], k: int, device, dtype):
+        self.projs = [name for name, _ in projs]
+        self.ends = []
+        for _, n in projs:
+            self.ends.append((self.ends[-1] if self.ends else 0) + n)
+        self.k = k
+        self.a = torch.zeros(0, 0, k, device=device, dtype=dtype)
+        self.b = torch.zeros(0, self.ends[-1], 0, device=device, dtype=dtype)
+
+    def resized(self, slots: int, rank: int):
+        S, R, P = self.b.shape[0], self.b.shape[2], len(self.ends)
+        a = self.a.new_zeros(slots, P, rank, self.k)
+        a[:S, :, :R] = self.a.view(S, P, R, self.k)
+        b = self.b.new_zeros(slots, self.ends[-1], rank)
+        b[:S, :, :R] = self.b
+        return a.view(slots, P * rank, self.k), b
+
+    def put(self, row: int, mods: dict) -> None:
+        """mods: proj -> (A, B)."""
+        R = self.b.shape[2]
+        self.a[row].zero_()
+        self.b[row].zero_()
+        first = 0
+        for p, (proj, end) in enumerate(zip(self.projs, self.ends)):
+            if proj in mods:
+                A, B = mods[proj]
+                self.a[row, p * R:p * R + A.shape[0]] = A
+                self.b[row, first:end, :B.shape[1]] = B
+            first = end
+
+
 class LoraBank:
-    """Registry of live adapters; slot 0 is reserved for "no adapter"."""
+    """Registry of live adapters; slot 0 is reserved for "no adapter". Slots
+    name adapters for good; rows of the stacked matrices are used again."""
 
     def __init__(self, spec, cfg):
         self.spec = spec
@@ -130,23 +170,100 @@ class LoraBank:
         self.adapters: dict[int, LoraAdapter] = {}
         self.by_name: dict[str, int] = {}
         self._next_slot = 1
+        self.row_of: dict[int, int] = {}     # slot -> row of the stacks
+        self._free: list[int] = []
+        # (layer, first projection) -> LoraGroup, where any adapter had one
+        self.groups: dict[tuple[int, str], LoraGroup] = {}
+        self.slots = 0                       # rows of the stacks
+        self.rank = 0                        # R, a multiple of 8
+        self.ranks: torch.Tensor | None = None   # int32 [slots]
+        self.version = 0                     # of the stacks' addresses
+
+    def _fused(self):
+        """First projection -> ([(projection, columns)], K) of this TP rank."""
+        spec, tp = self.spec, self.cfg.tp_size
+        d, h = spec.head_dim, spec.hidden_size
+        nq = spec.num_heads // tp * d
+        nk = max(1, spec.num_kv_heads // tp) * d
+        i = spec.intermediate_size // tp
+        up = [("up_proj", i)] if spec.mlp_no_gate else \
+            [("gate_proj", i), ("up_proj", i)]
+        return {"q_proj": ([("q_proj", nq), ("k_proj", nk), ("v_proj", nk)], h),
+                "o_proj": ([("o_proj", h)], nq),
+                up[0][0]: (up, h),
+                "down_proj": ([("down_proj", h)], i)}
 
     def add(self, name: str, adapter_dir: str, device, dtype) -> int:
         if name in self.by_name:
             return self.by_name[name]
         ad = LoraAdapter.load(name, adapter_dir, self.spec, self.cfg.tp_size,
                               self.cfg.tp_rank, device, dtype)
+        self._stack(self._next_slot, ad, device, dtype)
         slot = self._next_slot
         self._next_slot += 1
         self.adapters[slot] = ad
         self.by_name[name] = slot
         return slot
 
+    def _stack(self, slot: int, ad: LoraAdapter, device, dtype) -> None:
+        """The adapter's matrices into the stacks, which grow where they have
+        no row or rank for them: a growth gives all of them new addresses."""
+        fused = self._fused()
+        mods: dict[tuple[int, str], dict] = {}
+        rank = 0
+        for (li, proj), (A, B) in ad.mods.items():
+            first = next((f for f, (projs, _) in fused.items()
+                          if proj in dict(projs)), None)
+            if first is None:
+                raise ValueError(f"adapter {ad.name}: the model has no {proj}")
+            projs, k = fused[first]
+            n = dict(projs)[proj]
+            if A.shape[1] != k or B.shape != (n, A.shape[0]):
+                raise ValueError(
+                    f"adapter {ad.name}: {proj} of layer {li} is "
+                    f"{tuple(B.shape)} x {tuple(A.shape)}, not {n} x r x {k}")
+            rank = max(rank, A.shape[0])
+            mods.setdefault((li, first), {})[proj] = (A, B)
+        if self._free:
+            row, slots = self._free[-1], self.slots
+        else:
+            row = len(self.row_of)
+            slots = max(self.slots, 1 << row.bit_length())
+        new_rank = max(self.rank, (rank + 7) // 8 * 8)
+        grows = (slots, new_rank) != (self.slots, self.rank)
+        # all new memory first: an allocation that fails leaves the bank as it was
+        groups = dict(self.groups)
+        for key in mods:
+            if key not in groups:
+                groups[key] = LoraGroup(*fused[key[1]], device, dtype)
+        new = {key: g.resized(slots, new_rank) for key, g in groups.items()
+               if grows or key not in self.groups}
+        ranks = self.ranks
+        if grows:
+            ranks = torch.zeros(slots, dtype=torch.int32, device=device)
+            if self.ranks is not None:
+                ranks[:self.slots] = self.ranks
+        for key, (ga, gb) in new.items():
+            groups[key].a, groups[key].b = ga, gb
+        for key, g in groups.items():
+            g.put(row, mods.get(key, {}))
+        self.groups, self.ranks = groups, ranks
+        self.version += bool(new)
+        self.slots, self.rank = slots, new_rank
+        self.ranks[row:row + 1].fill_(rank)
+        if self._free:
+            self._free.pop()
+        self.row_of[slot] = row
+        ad.mods = {key: None for key in ad.mods}     # the stacks have them
+
     def remove(self, name: str) -> bool:
         slot = self.by_name.pop(name, None)
         if slot is None:
             return False
         self.adapters.pop(slot, None)
+        row = self.row_of.pop(slot)
+        self.ranks[row:row + 1].fill_(0)
+        self._free.append(row)
         return True
 
     def slot_of(self, name: str) -> int | None:
@@ -155,44 +272,50 @@ class LoraBank:
     def names(self) -> list[str]:
         return list(self.by_name)
 
+    def rows(self, row_slots: list[int]) -> list[int]:
+        """Rows of the stacks of a batch's slots, -1 without an adapter (none
+        was asked for, or it is gone)."""
+        return [self.row_of.get(s, -1) for s in row_slots]
+
 
 class BatchLora:
-    """Per-batch LoRA context: adapter row groups, precomputed host-side so
-    the per-layer apply is pure device work (no syncs on the hot path)."""
+    """Per-batch LoRA context: the rows adapter by adapter, precomputed host-side
+    so the per-layer apply is pure device work (no syncs on the hot path)."""
 
-    def __init__(self, bank: LoraBank, groups: list[tuple[int, torch.Tensor]]):
+    def __init__(self, bank: LoraBank, order: torch.Tensor,
+                 starts: torch.Tensor, counts: list[tuple[int, int, int]]):
         self.bank = bank
-        self.groups = groups  # [(slot, row-index tensor on device)]
+        self.order, self.starts = order, starts     # ops.build_lora_rows
+        self.counts = counts    # [(row of the stacks, first of order, number)]
 
     @classmethod
     def from_rows(cls, bank: LoraBank, row_slots: list[int], device):
-        groups: dict[int, list[int]] = {}
-        for i, s in enumerate(row_slots):
-            if s > 0:
-                groups.setdefault(s, []).append(i)
-        if not groups:
+        rows = bank.rows(row_slots)
+        if max(rows, default=-1) < 0:
             return None
-        return cls(bank, [
-            (slot, torch.tensor(rows, dtype=torch.long, device=device))
-            for slot, rows in sorted(groups.items())
-        ])
-
-    def _delta(self, A, B, x, rows):
-        xe = x.index_select(0, rows)
-        return torch.nn.functional.linear(
-            torch.nn.functional.linear(xe, A), B)
+        order, starts = ops.lora_rows(rows, bank.slots)
+        counts = [(i, int(starts[i]), int(starts[i + 1] - starts[i]))
+                  for i in range(bank.slots) if starts[i + 1] > starts[i]]
+        return cls(bank, *ops.to_device([(order, torch.int32),
+                                         (starts, torch.int32)], device), counts)
 
     def apply(self, li: int, x: torch.Tensor, out: torch.Tensor,
               projs: list[tuple[str, int, int]]) -> None:
         """out[rows, off:off+n] += lora_delta for each (proj, off, n)."""
-        for slot, rows in self.groups:
-            ad = self.bank.adapters.get(slot)
-            if ad is None:
-                continue
-            for proj, off, n in projs:
-                mod = ad.mods.get((li, proj))
-                if mod is None:
-                    continue
-                A, B = mod
-                d = self._delta(A, B, x, rows)
-                out[:, off:off + n].index_add_(0, rows, d)
+        g = self.bank.groups.get((li, projs[0][0]))
+        if g is None:
+            return
+        if ops.lora_add_ok(out, x, g.a, g.b, g.ends):
+            ops.lora_add(out, x, g.a, g.b, self.order, self.starts,
+                         self.bank.ranks, g.ends)
+            return
+        R = g.b.shape[2]
+        for row, first, n in self.counts:
+            rows = self.order[first:first + n].long()
+            xe, low = x.index_select(0, rows), 0
+            for p, end in enumerate(g.ends):
+                d = torch.nn.functional.linear(
+                    torch.nn.functional.linear(xe, g.a[row, p * R:(p + 1) * R]),
+                    g.b[row, low:end])
+                out[:, low:end].index_add_(0, rows, d)
+                low = end

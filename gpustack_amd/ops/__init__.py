@@ -2003,12 +2003,15 @@ def rows_fp8(x) -> Rows8:
     return Rows8(*k.fp8_rows(0, x, None, None, 0.0, False)[:2])
 
 
-def silu_and_mul_fp8(x) -> Rows8:
-    """silu(gate) * up of x = [gate | up] in 8 bits, rounded once."""
+def silu_and_mul_fp8(x, rows: bool = False) -> Rows8:
+    """silu(gate) * up of x = [gate | up] in 8 bits, rounded once. `rows`: in
+    x's type too."""
     k = _fp8_backend(x)
     if k is None:
-        return Rows8(*torch_ref.silu_and_mul_fp8(x))
-    return Rows8(*k.fp8_rows(1, x, None, None, 0.0, False)[:2])
+        q, scale, act = torch_ref.silu_and_mul_fp8(x)
+        return Rows8(q, scale, act if rows else None)
+    q, scale, _, act = k.fp8_rows(1, x, None, None, 0.0, rows)
+    return Rows8(q, scale, act)
 
 
 def add_rms_norm_fp8(x, residual, weight, eps: float, rows: bool = False):
@@ -2144,6 +2147,18 @@ def lora_rows(slots, n_slots: int):
     order = np.argsort(key, kind="stable").astype(np.int32)
     starts = np.searchsorted(key[order], np.arange(n_slots + 1)).astype(np.int32)
     return order, starts
+
+
+def lora_add_ok(out, x, a, b, ends) -> bool:
+    """Operands that lora_add takes, by type, sizes and places."""
+    R = b.shape[2]
+    return (0 < R <= 256 and R % 8 == 0 and a.shape[2] % 8 == 0
+            and all(e % 8 == 0 for e in ends) and len(ends) <= 4
+            and x.dim() == out.dim() == 2
+            and (not x.is_cuda or all(
+                t.dtype == torch.bfloat16 and t.data_ptr() % 16 == 0
+                and t.stride(-1) == 1 and t.stride(0) % 8 == 0
+                for t in (out, x, a, b))))
 
 
 def lora_add(out, x, a, b, order, starts, ranks, ends) -> None:

@@ -61,7 +61,7 @@ long chk_rows(const Tensor& t, const char* name, const Tensor& like) {
 }
 
 // (q, scale, sum, rows): source 0 x as it is, 1 silu(gate) * up, 2 the norm of
-// x + residual, whose sum comes too, or of x; `keep`: the norm in bf16 as well
+// x + residual, whose sum comes too, or of x; `keep` (1, 2): the rows in bf16 as well
 std::tuple<Tensor, Tensor, OptTensor, OptTensor> fp8_rows(
     int64_t source, Tensor x, OptTensor residual, OptTensor weight, double eps,
     bool keep) {
@@ -72,8 +72,8 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> fp8_rows(
               (source != 1 || W % 2 == 0),
               "fp8_rows: rows of ", W, " elements: the result's are a multiple of 8, at most ",
               fp8_rows_most());
-  TORCH_CHECK(weight.has_value() == (source == 2) && (source == 2 || !(residual || keep)),
-              "fp8_rows: what belongs to the norm");
+  TORCH_CHECK(weight.has_value() == (source == 2) && (source == 2 || !residual) &&
+              (source > 0 || !keep), "fp8_rows: what belongs to the norm");
   if (weight) {
     chk(*weight, "weight", at::kBFloat16, x);
     TORCH_CHECK(weight->dim() == 1 && weight->size(0) == H, "fp8_rows: weight's size");

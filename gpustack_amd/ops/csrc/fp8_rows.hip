@@ -38,7 +38,7 @@ template <int SRC, int G, int NV>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
     unsigned char* __restrict__ q, float* __restrict__ scale,
     unsigned short* __restrict__ sum,        // NORM: x + residual, with a residual
-    unsigned short* __restrict__ rows,       // NORM: v in bf16, or null
+    unsigned short* __restrict__ rows,       // NORM, SILU: v in bf16, or null
     const unsigned short* __restrict__ x, long xs,
     const unsigned short* __restrict__ residual,
     const unsigned short* __restrict__ weight, float eps, int T, int H) {
@@ -62,6 +62,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           v[i][j] = over_one_plus_exp(bf2f(a[j]), bf2f(a[j])) * bf2f(b[j]);
+        if (rows) *reinterpret_cast<u16x8*>(rows + row * H + c) = f32_to_bf8(v[i]);
       } else {
         u16x8 r = a;
         if (SRC == NORM && residual) {

@@ -1154,9 +1154,11 @@ def fp8_rows(v: torch.Tensor):
 
 
 def silu_and_mul_fp8(x: torch.Tensor):
+    """(e4m3 rows, scales, the rows in x's type)."""
     _want(x.dim() == 2 and x.shape[1] % 2 == 0, "fp8_rows: [gate | up] rows")
     g, u = x.float().chunk(2, 1)
-    return fp8_rows(g / (1 + torch.exp(-g)) * u)
+    v = g / (1 + torch.exp(-g)) * u
+    return *fp8_rows(v), v.to(x.dtype)
 
 
 def add_rms_norm_fp8(x, residual, weight, eps: float):

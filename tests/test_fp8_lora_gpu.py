@@ -41,7 +41,12 @@ def test_rows(width, rows):
     d = g.double()
     v = d[:, :width] * torch.sigmoid(d[:, :width]) * d[:, width:]
     # over_one_plus_exp is within 1.34e-7 of the quotient, a product behind it
-    _check_rows(ops.silu_and_mul_fp8(g), v, 2 ** -21)
+    r = ops.silu_and_mul_fp8(g)
+    _check_rows(r, v, 2 ** -21)
+    both = ops.silu_and_mul_fp8(g, rows=True)
+    assert r.rows is None and torch.equal(both.scale, r.scale)
+    assert torch.equal(both.q.float(), r.q.float())
+    assert ((both.rows.double() - v).abs() <= v.abs() * (2 ** -8 + 2 ** -20)).all()
 
 
 @pytest.mark.parametrize("width", WIDTHS)

@@ -1,0 +1,185 @@
+"""The adapters' stacked matrices and what a batch adds with them."""
+import json
+
+import pytest
+import torch
+from safetensors.torch import save_file
+
+from gpustack_amd.engine import EngineConfig, LLMEngine, SamplingParams
+from gpustack_amd.models.lora import BatchLora, LoraBank
+
+GPU = pytest.param("cuda", marks=[
+    pytest.mark.gpu,
+    pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")])
+
+
+def sizes(spec):
+    d, h, i = spec.head_dim, spec.hidden_size, spec.intermediate_size
+    nq, nk = spec.num_heads * d, spec.num_kv_heads * d
+    return {"q_proj": (nq, h), "k_proj": (nk, h), "v_proj": (nk, h),
+            "o_proj": (h, nq), "gate_proj": (i, h), "up_proj": (i, h),
+            "down_proj": (h, i)}
+
+
+def make(path, spec, seed, r, projs, alpha=8, layers=None):
+    """An adapter's files; its matrices by (layer, projection), alpha / r in B."""
+    g = torch.Generator().manual_seed(seed)
+    tensors, mods = {}, {}
+    for li in layers if layers is not None else range(spec.num_layers):
+        for proj in projs:
+            n, k = sizes(spec)[proj]
+            A = torch.randn(r, k, generator=g) * k ** -.5
+            B = torch.randn(n, r, generator=g) * .3
+            part = "self_attn" if proj[0] in "qkvo" and proj != "up_proj" else "mlp"
+            pre = f"base_model.model.model.layers.{li}.{part}.{proj}"
+            tensors[f"{pre}.lora_A.weight"] = A
+            tensors[f"{pre}.lora_B.weight"] = B
+            mods[li, proj] = A, B * (alpha / r)
+    path.mkdir()
+    save_file(tensors, str(path / "adapter_model.safetensors"))
+    (path / "adapter_config.json").write_text(json.dumps({"r": r, "lora_alpha": alpha}))
+    return mods
+
+
+PROJS = {"qkv": [("q_proj",), ("k_proj",), ("v_proj",)], "o": [("o_proj",)],
+         "gu": [("gate_proj",), ("up_proj",)], "down": [("down_proj",)]}
+
+
+def check(bank, known, row_slots, spec, device, dtype):
+    """Every projection of every layer against the adapters' own matrices."""
+    g = torch.Generator().manual_seed(len(row_slots))
+    batch = BatchLora.from_rows(bank, row_slots, device)
+    live = [s if s in known else 0 for s in row_slots]
+    if not any(live):
+        assert batch is None
+        return
+    eps = torch.finfo(dtype).eps
+    for li in range(spec.num_layers):
+        for names in PROJS.values():
+            projs, off = [], 0
+            for (name,) in names:
+                n, k = sizes(spec)[name]
+                projs.append((name, off, n))
+                off += n
+            x = torch.randn(len(row_slots), k, generator=g).to(dtype)
+            out = torch.randn(len(row_slots), off, generator=g).to(dtype)
+            want, size = out.double(), torch.zeros(out.shape, dtype=torch.float64)
+            for t, s in enumerate(live):
+                for name, first, n in projs:
+                    if s and (li, name) in known[s]:
+                        A, B = (m.to(dtype).double() for m in known[s][li, name])
+                        want[t, first:first + n] += B @ (A @ x[t].double())
+                        size[t, first:first + n] = \
+                            B.abs() @ (A.abs() @ x[t].double().abs())
+            got = out.to(device)
+            batch.apply(li, x.to(device), got, projs)
+            # one rounding; fp32 sums, the middle values in two bf16 parts
+            assert ((got.cpu().double() - want).abs()
+                    <= want.abs() * (eps / 2 + 2 ** -20) + size * 2 ** -15).all()
+            for t, s in enumerate(live):
+                if not s:
+                    assert torch.equal(got[t].cpu(), out[t])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_stacks_grow_and_are_used_again(tmp_path, device, dtype):
+    cfg = EngineConfig(model="tiny", device="cpu")
+    spec, bank = cfg.spec, LoraBank(cfg.spec, cfg)
+    known = {}
+
+    def add(name, **kw):
+        mods = make(tmp_path / name, spec, **kw)
+        slot = bank.add(name, str(tmp_path / name), device, dtype)
+        known[slot] = mods
+        return slot
+
+    a = add("a", seed=1, r=4, projs=["q_proj", "down_proj"])
+    assert (bank.slots, bank.rank) == (1, 8)
+    check(bank, known, [a, 0, a], spec, device, dtype)
+    before = bank.version
+    b = add("b", seed=2, r=20, projs=["k_proj", "v_proj", "o_proj", "up_proj"])
+    assert (bank.slots, bank.rank) == (2, 24) and bank.version > before
+    check(bank, known, [b, a, 0, b, a], spec, device, dtype)
+    c = add("c", seed=3, r=3, projs=["gate_proj", "q_proj"], layers=[1])
+    assert bank.slots == 4
+    check(bank, known, [c, b, a, 0], spec, device, dtype)
+    # a removed adapter's row is free, its slot names nothing any more
+    assert bank.remove("b") and not bank.remove("b")
+    known.pop(b)
+    check(bank, known, [c, b, a, 0], spec, device, dtype)
+    check(bank, known, [b, b], spec, device, dtype)
+    before = bank.version
+    e = add("e", seed=4, r=8, projs=["v_proj", "down_proj"])
+    assert bank.slots == 4 and bank.row_of[e] == 1 and bank.version == before
+    check(bank, known, [e, b, c, a, e, 0], spec, device, dtype)
+    assert bank.add("e", "nowhere", device, dtype) == e
+
+
+def test_refused_adapters_leave_the_bank(tmp_path):
+    cfg = EngineConfig(model="tiny", device="cpu")
+    bank = LoraBank(cfg.spec, cfg)
+    make(tmp_path / "good", cfg.spec, 1, 4, ["q_proj"])
+    bank.add("good", str(tmp_path / "good"), "cpu", torch.float32)
+    other = EngineConfig(model="tiny", device="cpu").spec
+    other.hidden_size += 16
+    make(tmp_path / "bad", other, 1, 64, ["q_proj"])
+    state = (bank.slots, bank.rank, bank.version, dict(bank.row_of))
+    with pytest.raises(ValueError, match="q_proj of layer 0"):
+        bank.add("bad", str(tmp_path / "bad"), "cpu", torch.float32)
+    assert (bank.slots, bank.rank, bank.version, bank.row_of) == state
+    assert bank.names() == ["good"] and bank.slot_of("bad") is None
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_ranks_that_the_kernel_does_not_take(tmp_path, device):
+    cfg = EngineConfig(model="tiny", device="cpu")
+    bank = LoraBank(cfg.spec, cfg)
+    mods = make(tmp_path / "wide", cfg.spec, 1, 264, ["q_proj", "o_proj"])
+    slot = bank.add("wide", str(tmp_path / "wide"), device, torch.float32)
+    known = {slot: mods}
+    g = torch.Generator().manual_seed(1)
+    batch = BatchLora.from_rows(bank, [0, slot, slot], device)
+    n, k = sizes(cfg.spec)["o_proj"]
+    x, out = torch.randn(3, k, generator=g), torch.randn(3, n, generator=g)
+    A, B = known[slot][0, "o_proj"]
+    want = out.clone()
+    want[1:] += x[1:] @ A.T @ B.T
+    got = out.to(device)
+    batch.apply(0, x.to(device), got, [("o_proj", 0, n)])
+    assert torch.allclose(got.cpu(), want, rtol=1e-4, atol=1e-4)
+
+
+def test_engine_with_adapters_that_come_and_go(tmp_path):
+    """Rows keep to their own adapter while others are loaded and removed."""
+    spec = EngineConfig(model="tiny").spec
+    projs = list(sizes(spec))
+    for name, r in (("a", 4), ("b", 12), ("c", 6)):
+        make(tmp_path / name, spec, ord(name), r, projs)
+
+    def params(name=None):
+        return SamplingParams(max_tokens=6, ignore_eos=True, lora_name=name)
+
+    def engine(**kw):
+        return LLMEngine(EngineConfig(model="tiny", device="cpu",
+                                      kv_cache_blocks=64, **kw))
+
+    prompt = [1, 2, 3, 4, 5]
+    solo = {}
+    for name in "abc":
+        e = engine()
+        e.add_lora(name, str(tmp_path / name))
+        solo[name] = e.generate([prompt], params(name))[0]
+    assert len({tuple(v) for v in solo.values()}) == 3
+    e = engine()
+    for name in "ab":
+        e.add_lora(name, str(tmp_path / name))
+    assert e.generate([prompt], params("b"))[0] == solo["b"]
+    assert e.remove_lora("a")
+    e.add_lora("c", str(tmp_path / "c"))
+    ids = {n: e.add_request(prompt, params(n)) for n in "bc"}
+    got = {i: [] for i in ids.values()}
+    while e.has_unfinished():
+        for o in e.step():
+            got[o.request_id].append(o.token_id)
+    assert got[ids["b"]] == solo["b"] and got[ids["c"]] == solo["c"]
