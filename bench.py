@@ -44,8 +44,9 @@ def parse_args():
                          "scripts/train_eagle_draft.py)")
     ap.add_argument("--prefix-caching", action="store_true",
                     help="enable automatic prefix caching (shared-prefix workloads)")
-    ap.add_argument("--quantize", default=None, choices=["w4"],
-                    help="runtime weight quantization (packed int4 in HBM)")
+    ap.add_argument("--quantize", default=None, choices=["w4", "fp8"],
+                    help="runtime weight quantization (packed int4, or e4m3 "
+                         "with rows in 8 bits)")
     ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "fp8"],
                     help="KV cache dtype (fp8 e4m3 halves KV bytes; compute stays bf16)")
     ap.add_argument("--device", default=None)
@@ -276,7 +277,7 @@ def main():
             "higher_is_better": True,
             "scaling": "strong" if comm is not None else "weak",
             "vs_baseline": None,
-            "dtype": (f"{cfg.dtype}+w4-weights" if args.quantize == "w4"
+            "dtype": (f"{cfg.dtype}+{args.quantize}-weights" if args.quantize
                       else cfg.dtype) if use_cuda else "float32-cpu-smoke",
             "data": "synthetic random-token prompts, random-init weights",
             "config": {

@@ -1735,7 +1735,9 @@ class EngineConfig:
     # W4 runtime quantization ("w4"): the big serving weights are packed
     # int4 in HBM after load and decode GEMMs dequantize in-register
     # (ops/csrc/w4_gemm.hip) — 70B-class models stay resident packed
-    # instead of inflating to bf16 (reference: vLLM --quantization)
+    # instead of inflating to bf16 (reference: vLLM --quantization).
+    # "fp8": dense projections in e4m3, their rows brought to 8 bits on the
+    # way (ops/csrc/fp8_gemm.hip, fp8_wide.hip)
     quantize_runtime: str | None = None
     # CPU weight offload (reference: vLLM --cpu-offload-gb, the GGUF
     # partial-offload placement): ~this many GiB of trailing layers'

@@ -289,6 +289,14 @@ class ModelRunner:
 
             logging.getLogger(__name__).info(
                 "W4 runtime: %d weight tensors packed int4", n)
+        elif getattr(cfg, "quantize_runtime", None) == "fp8":
+            from ..models.weights import convert_to_fp8_runtime
+
+            n = convert_to_fp8_runtime(self.model, cfg)
+            import logging
+
+            logging.getLogger(__name__).info(
+                "fp8 runtime: %d weight tensors in e4m3", n)
         if getattr(cfg, "cpu_offload_gb", 0) > 0:
             from .offload import setup_cpu_offload
 

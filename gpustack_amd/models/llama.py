@@ -210,8 +210,21 @@ class W4Pack:
         self.shape = (qw.shape[0], qw.shape[1] * 2)
 
 
-def qlinear(x, w, pack: "W4Pack | None", bias=None, parts: bool = False):
-    """F.linear with an optional W4 runtime pack. `parts` as in
+class F8Pack:
+    """e4m3 weight (models/weights.py convert_to_fp8_runtime): q [N, K], a
+    fp32 scale a column, and the type of its products."""
+
+    __slots__ = ("q", "scale", "dtype", "shape")
+
+    def __init__(self, q, scale, dtype):
+        self.q, self.scale, self.dtype = q, scale, dtype
+        self.shape = tuple(q.shape)
+
+
+def qlinear(x, w, pack: "W4Pack | F8Pack | None", bias=None,
+            parts: bool = False):
+    """F.linear with an optional W4 runtime pack, or of e4m3 weights: x is
+    brought to 8 bits unless it is already (ops.Rows8). `parts` as in
     ops.linear_auto.
 
     Packed weights stay RESIDENT packed (the capacity goal). Up to 192 rows
@@ -227,6 +240,9 @@ def qlinear(x, w, pack: "W4Pack | None", bias=None, parts: bool = False):
     if pack is None:
         return ops.linear_auto(x, w, parts) if bias is None \
             else F.linear(x, w, bias)
+    if isinstance(pack, F8Pack):
+        r = x if isinstance(x, ops.Rows8) else ops.rows_fp8(x.contiguous())
+        return ops.linear_fp8(r.q, r.scale, pack.q, pack.scale, bias, pack.dtype)
     if x.is_cuda:
         hip = ops._load_hip()
         if _w4_takes(x, pack):
@@ -261,11 +277,13 @@ def _w4_takes(x, pack: "W4Pack") -> bool:
             and N % 64 == 0 and K <= 131072)
 
 
-def _gate_up_silu(x, w, pack: "W4Pack | None"):
+def _gate_up_silu(x, w, pack: "W4Pack | F8Pack | None"):
     """silu(gate) * up of the fused product where it ends in the activation,
     else None."""
     if pack is None:
         return ops.linear_silu(x, w)
+    if isinstance(pack, F8Pack):
+        return None
     hip = ops._load_hip() if _w4_takes(x, pack) else None
     if hip is None or not hip.w4_silu_wins(x.shape[0], *pack.shape):
         return None
@@ -316,8 +334,8 @@ class Attention(nn.Module):
             self.window = spec.sliding_window if sliding else 0
         else:
             self.window = 0
-        self.qkv_pack: W4Pack | None = None   # W4 runtime (qlinear)
-        self.o_pack: W4Pack | None = None
+        self.qkv_pack: W4Pack | F8Pack | None = None   # qlinear
+        self.o_pack: W4Pack | F8Pack | None = None
         self.layer_idx = 0  # set by LlamaForCausalLM
         nq, nk = self.hq * self.d, self.hkv * self.d
         self._qkv_projs = [("q_proj", 0, nq), ("k_proj", nq, nk),
@@ -339,24 +357,29 @@ class Attention(nn.Module):
 
     def forward(self, x, meta: ForwardMeta, cos_sin, k_cache, v_cache,
                 parts: bool = False):
-        """`parts`: the result may be the parts of the output product
+        """x: rows, or in 8 bits (ops.Rows8) where the projection's weights
+        are. `parts`: the result may be the parts of the output product
         (ops.linear_auto)."""
-        T = x.shape[0]
+        eight = isinstance(x, ops.Rows8)
+        T = x[0].shape[0] if eight else x.shape[0]
         head_norm = self.spec.qk_norm and not (
             self.spec.qk_norm_full or self.spec.qk_norm_after_rope)
         store = (meta.cp is None and self.use_rope
                  and (head_norm or not self.spec.qk_norm))
         qkv = qlinear(x, self.qkv_w, self.qkv_pack, self.qkv_b,
-                      parts=store and meta.lora is None and ops.qkv_store_ok(
-                          x, self.d, self.rot_dim, self.spec.rope_mode))
+                      parts=store and meta.lora is None and not eight
+                      and ops.qkv_store_ok(x, self.d, self.rot_dim,
+                                           self.spec.rope_mode))
+        like = qkv if eight else x       # the rows' type and device
         norms = (self.q_norm, self.k_norm) if head_norm else (None, None)
         if store and meta.own_rows and meta.lora is None \
                 and not (self.sinks is not None or self.window or self.softcap) \
-                and ops.qkv_store_ok(x, self.d, self.rot_dim, self.spec.rope_mode) \
-                and ops.paged_attn_decode_rows_ok(x, self.hq, self.hkv, self.d,
+                and ops.qkv_store_ok(like, self.d, self.rot_dim, self.spec.rope_mode) \
+                and ops.paged_attn_decode_rows_ok(like, self.hq, self.hkv, self.d,
                                                   k_cache, v_cache,
                                                   meta.block_tables, *norms):
-            out = torch.empty(T, self.hq, self.d, dtype=x.dtype, device=x.device)
+            out = torch.empty(T, self.hq, self.d, dtype=like.dtype,
+                              device=like.device)
             ops.paged_attn_decode_rows(
                 out, qkv, self.hq, self.hkv, *norms, cos_sin, meta.positions,
                 meta.slot_mapping, k_cache, v_cache, meta.block_tables,
@@ -370,7 +393,8 @@ class Attention(nn.Module):
             qkv = torch.empty(qkv.shape[1:], dtype=x.dtype, device=x.device)
         if meta.lora is not None:
             qkv = qkv.contiguous()
-            meta.lora.apply(self.layer_idx, x, qkv, self._qkv_projs)
+            meta.lora.apply(self.layer_idx, x.rows if eight else x, qkv,
+                            self._qkv_projs)
         nq, nk = self.hq * self.d, self.hkv * self.d
         # strided views into the fused buffer — the HIP kernels take row
         # strides, so no layout copies on the hot path
@@ -735,8 +759,8 @@ class MLP(nn.Module):
         gu_rows = self.i if self.no_gate else 2 * self.i
         self.gate_up_w = nn.Parameter(torch.empty(gu_rows, h, dtype=dtype), requires_grad=False)
         self.down_w = nn.Parameter(torch.empty(h, self.i, dtype=dtype), requires_grad=False)
-        self.gate_up_pack: W4Pack | None = None  # W4 runtime (qlinear)
-        self.down_pack: W4Pack | None = None
+        self.gate_up_pack: W4Pack | F8Pack | None = None  # qlinear
+        self.down_pack: W4Pack | F8Pack | None = None
         self.layer_idx = 0  # set by LlamaForCausalLM
         self._gu_projs = ([("up_proj", 0, self.i)] if self.no_gate else
                           [("gate_proj", 0, self.i), ("up_proj", self.i, self.i)])
@@ -754,13 +778,17 @@ class MLP(nn.Module):
         down = qlinear(act, self.down_w, self.down_pack,
                        parts=parts and not lora)
         if lora:
-            meta.lora.apply(self.layer_idx, act, down, self._down_projs)
+            meta.lora.apply(self.layer_idx,
+                            act.rows if isinstance(act, ops.Rows8) else act,
+                            down, self._down_projs)
         return self.comm.all_reduce(down)
 
     def _activated(self, x, meta):
         gu = qlinear(x, self.gate_up_w, self.gate_up_pack)
         if meta is not None:
-            meta.lora.apply(self.layer_idx, x, gu, self._gu_projs)
+            meta.lora.apply(self.layer_idx,
+                            x.rows if isinstance(x, ops.Rows8) else x, gu,
+                            self._gu_projs)
         if self.no_gate:
             # Arcee: single up projection, relu^2 activation
             act = (torch.square(F.relu(gu)) if self.act == "relu2"
@@ -771,9 +799,12 @@ class MLP(nn.Module):
             # GPT-OSS clamped-swiglu kernel work)
             act = (F.gelu(gu[:, :self.i], approximate="tanh")
                    * gu[:, self.i:])
+        elif isinstance(self.down_pack, F8Pack):
+            # (adapters read the rows)
+            return ops.silu_and_mul_fp8(gu, rows=meta is not None)
         else:
-            act = torch.empty(x.shape[0], self.i, dtype=x.dtype,
-                              device=x.device)
+            act = torch.empty(gu.shape[0], self.i, dtype=gu.dtype,
+                              device=gu.device)
             ops.silu_and_mul(act, gu)
         return act
 
@@ -1287,26 +1318,38 @@ class DecoderLayer(nn.Module):
         if self.spec.norm_after:
             return self._forward_norm_after(x, meta, cos_sin, k_cache,
                                             v_cache, eps)
-        if residual is None:
-            residual = x
-            h = normed
-            if h is None:
-                h = torch.empty_like(x)
-                ops.rms_norm(h, x, self.input_norm, eps)
+        lora = meta.lora is not None    # adapters read the rows themselves
+        if normed is not None and residual is None:
+            h, residual = normed, x
         else:
-            h = ops.add_rms_norm(x, residual, self.input_norm, eps)
+            h, residual = self._norm(x, residual, self.input_norm, self.attn,
+                                     "qkv_pack", lora)
         rm = self.spec.residual_multiplier
         kw = {"parts": True} if parts and not rm else {}
         a = self.attn(h, meta, cos_sin, k_cache, v_cache,
                       **(kw if isinstance(self.attn, Attention) else {}))
         if rm:  # Granite: scale sublayer outputs before the residual add
             a = a * rm
-        a = ops.add_rms_norm(a, residual, self.post_attn_norm, eps)
+        a, residual = self._norm(a, residual, self.post_attn_norm, self.mlp,
+                                 "gate_up_pack", lora)
         m = self.mlp(a, meta, **(kw if isinstance(self.mlp, (MLP, MoEMLP))
                                 else {}))
         if rm:
             m = m * rm
         return m, residual
+
+    def _norm(self, x, residual, weight, module, pack: str, rows: bool):
+        """(the norm of x + residual, the sum): in 8 bits where the first
+        product behind it takes them (`module`'s `pack`), with `rows` in x's
+        type too."""
+        eps = self.spec.rms_norm_eps
+        if x.dim() == 2 and isinstance(getattr(module, pack, None), F8Pack):
+            return ops.add_rms_norm_fp8(x, residual, weight, eps, rows=rows)
+        if residual is None:
+            h = torch.empty_like(x)
+            ops.rms_norm(h, x, weight, eps)
+            return h, x
+        return ops.add_rms_norm(x, residual, weight, eps), residual
 
     def _forward_parallel(self, x, meta, cos_sin, k_cache, v_cache, eps):
         """Cohere layer flow (true hidden stream, residual sentinel

@@ -1183,3 +1183,40 @@ def convert_to_w4_runtime(model, cfg: EngineConfig) -> int:
     if model.device.type == "cuda":
         torch.cuda.empty_cache()
     return n_packed
+
+
+def convert_to_fp8_runtime(model, cfg: EngineConfig) -> int:
+    """Bring the layers' dense projections to e4m3 with a scale a column and
+    free their parameters: rows come to their products in 8 bits as well
+    (ops.add_rms_norm_fp8, silu_and_mul_fp8, rows_fp8; ops.linear_fp8). The
+    embedding and the head keep their type, as do expert banks, latent
+    attention and widths that the products do not take (N % 8, K % 16).
+    Returns the number of converted tensors. Reference capability: vLLM
+    --quantization fp8 with dynamic activation scales.
+    """
+    from .. import ops
+    from .llama import Attention, F8Pack, MLP
+
+    if model.device.type == "cuda" and cfg.dtype != "bfloat16":
+        raise ValueError("quantize_runtime fp8 serves bfloat16 models on the "
+                         f"GPU, not {cfg.dtype}")
+    n = 0
+    for layer in model.layers:
+        for mod, kind, sites in (
+                (layer.attn, Attention, (("qkv_w", "qkv_pack"), ("o_w", "o_pack"))),
+                (layer.mlp, MLP, (("gate_up_w", "gate_up_pack"),
+                                  ("down_w", "down_pack")))):
+            if not isinstance(mod, kind):
+                continue
+            for wname, pname in sites:
+                w = getattr(mod, wname)
+                if w.numel() == 0 or w.shape[0] % 8 or w.shape[1] % 16 \
+                        or w.shape[1] > 65536:
+                    continue
+                r = ops.rows_fp8(w.data)
+                setattr(mod, pname, F8Pack(r.q, r.scale, w.dtype))
+                w.data = torch.empty(0, dtype=w.dtype, device=w.device)
+                n += 1
+    if model.device.type == "cuda":
+        torch.cuda.empty_cache()
+    return n

@@ -81,11 +81,17 @@ def model_spec_for(model: Model | dict) -> ModelSpec | None:
 def _weight_bytes(model: dict, spec: ModelSpec, tp: int) -> int:
     """Per-shard resident weight bytes, accounting for runtime W4 packing
     (backend_parameters quantize_runtime=w4 keeps weights int4: ~0.28x of
-    bf16 incl. scales) and the bf16 default."""
+    bf16 incl. scales), e4m3 layers (quantize_runtime=fp8; embedding, head,
+    experts and latent attention keep theirs) and the bf16 default."""
     bp = model.get("backend_parameters") or {}
     w = spec.weight_bytes() // tp
     if bp.get("quantize_runtime") == "w4":
         w = int(w * 0.28)
+    elif (bp.get("quantize_runtime") == "fp8" and not spec.num_experts
+          and not spec.kv_lora_rank and spec.layers is None):
+        rest = spec.vocab_size * spec.hidden_size * 2 // tp \
+            * (1 if spec.tie_word_embeddings else 2)
+        w = rest + int(max(w - rest, 0) * 0.51)
     return w
 
 

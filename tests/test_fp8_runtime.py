@@ -1,0 +1,115 @@
+"""quantize_runtime="fp8": e4m3 projections, rows brought to 8 bits on the way."""
+import pytest
+import torch
+
+from gpustack_amd import ops
+from gpustack_amd.engine import EngineConfig, LLMEngine, SamplingParams
+from gpustack_amd.engine.config import ModelSpec
+from gpustack_amd.models.llama import F8Pack, qlinear
+from gpustack_amd.scheduler.policies import _weight_bytes
+from test_lora_bank import make, sizes
+
+P = SamplingParams(max_tokens=6, ignore_eos=True)
+
+
+def engine(model="tiny", **kw):
+    return LLMEngine(EngineConfig(model=model, device="cpu", kv_cache_blocks=64, **kw))
+
+
+def test_projections_are_converted():
+    model = engine(quantize_runtime="fp8").runner.model
+    for layer in model.layers:
+        for mod, w, pack in ((layer.attn, "qkv_w", "qkv_pack"),
+                             (layer.attn, "o_w", "o_pack"),
+                             (layer.mlp, "gate_up_w", "gate_up_pack"),
+                             (layer.mlp, "down_w", "down_pack")):
+            p = getattr(mod, pack)
+            assert isinstance(p, F8Pack) and p.q.dtype == torch.float8_e4m3fn
+            assert getattr(mod, w).numel() == 0
+    assert model.lm_head_pack is None and model.lm_head.numel() > 0
+
+
+@pytest.mark.parametrize("model", ["tiny", "tiny-moe", "tiny-mla"])
+def test_engine_serves(model):
+    out = engine(model, quantize_runtime="fp8").generate([[1, 2, 3, 4]], P)[0]
+    assert len(out) == 6
+    assert engine(model, quantize_runtime="fp8").generate([[1, 2, 3, 4]], P)[0] == out
+
+
+def test_one_layer_is_the_products_of_its_rounded_operands():
+    """What a layer computes, step by step, from the rounded weights and rows."""
+    from gpustack_amd.models.llama import ForwardMeta
+
+    cfg = EngineConfig(model="tiny", device="cpu", kv_cache_blocks=64,
+                       quantize_runtime="fp8")
+    run = LLMEngine(cfg).runner
+    layer, spec = run.model.layers[0], cfg.spec
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(5, spec.hidden_size, generator=g).to(run.model.dtype)
+    res = torch.randn(5, spec.hidden_size, generator=g).to(run.model.dtype)
+    meta = ForwardMeta(is_prefill=True, positions=torch.arange(5),
+                       slot_mapping=torch.full((5,), -1),
+                       logits_indices=torch.tensor([4]), seq_lens_list=[5],
+                       block_tables=None)
+    k, v = run.kv.k_caches[0], run.kv.v_caches[0]
+    m, total = layer(x.clone(), res.clone(), meta, run.model.cos_sin, k, v)
+
+    def product(rows, pack):
+        q, s, _ = ops.rows_fp8(rows)
+        w = pack.q.float() * pack.scale[:, None]
+        return ((q.float() * s[:, None]) @ w.T).to(pack.dtype)
+
+    eps = spec.rms_norm_eps
+    r1, t1 = ops.add_rms_norm_fp8(x, res, layer.input_norm, eps)
+    plain = r1.q.float() * r1.scale[:, None]
+    packs = layer.attn, layer.mlp
+    got_qkv = qlinear(r1, None, packs[0].qkv_pack)
+    want_qkv = (plain @ (packs[0].qkv_pack.q.float()
+                         * packs[0].qkv_pack.scale[:, None]).T)
+    assert torch.allclose(got_qkv.float(), want_qkv, rtol=1e-2, atol=1e-3)
+    a = layer.attn(r1, meta, run.model.cos_sin, k, v)
+    r2, t2 = ops.add_rms_norm_fp8(a, t1, layer.post_attn_norm, eps)
+    gu = qlinear(r2, None, packs[1].gate_up_pack)
+    act = ops.silu_and_mul_fp8(gu)
+    down = qlinear(act, None, packs[1].down_pack)
+    assert torch.equal(down, m) and torch.equal(t2, total)
+    # rows that are not in 8 bits yet are brought there
+    assert torch.equal(qlinear(x, None, packs[0].qkv_pack), product(x, packs[0].qkv_pack)) \
+        or torch.allclose(qlinear(x, None, packs[0].qkv_pack).float(),
+                          product(x, packs[0].qkv_pack).float(), rtol=2 ** -7, atol=1e-4)
+
+
+def test_near_the_unconverted_engine():
+    """Hidden states of 8-bit layers stay near: an e4m3 product's terms are off
+    by up to 2^-4 on both sides, at random, so a sum of them by far less than
+    an eighth of its size."""
+    a, b = engine(), engine(quantize_runtime="fp8")
+    e = [r.runner.embed([[1, 2, 3, 4, 5, 6, 7, 8]])[0] for r in (a, b)]
+    x, y = torch.tensor(e[0]), torch.tensor(e[1])
+    assert (x - y).norm() < .125 * x.norm()
+
+
+def test_adapters_beside_8_bit_projections(tmp_path):
+    spec = EngineConfig(model="tiny").spec
+    make(tmp_path / "a", spec, 3, 8, list(sizes(spec)))
+    e = engine(quantize_runtime="fp8")
+    base = e.generate([[1, 2, 3, 4, 5]], P)[0]
+    e.add_lora("a", str(tmp_path / "a"))
+    with_a = SamplingParams(max_tokens=6, ignore_eos=True, lora_name="a")
+    ids = [e.add_request([1, 2, 3, 4, 5], p) for p in (P, with_a)]
+    got = {i: [] for i in ids}
+    while e.has_unfinished():
+        for o in e.step():
+            got[o.request_id].append(o.token_id)
+    assert got[ids[0]] == base and got[ids[1]] != base
+
+
+def test_memory_of_a_converted_model():
+    spec = ModelSpec()
+    w = spec.weight_bytes()
+    got = _weight_bytes({"backend_parameters": {"quantize_runtime": "fp8"}}, spec, 1)
+    rest = spec.vocab_size * spec.hidden_size * 2 * (1 if spec.tie_word_embeddings else 2)
+    assert rest + (w - rest) // 2 < got < w
+    moe = EngineConfig(model="tiny-moe").spec
+    assert _weight_bytes({"backend_parameters": {"quantize_runtime": "fp8"}}, moe, 1) \
+        == moe.weight_bytes()
