@@ -177,7 +177,6 @@ class LoraBank:
         self.slots = 0                       # rows of the stacks
         self.rank = 0                        # R, a multiple of 8
         self.ranks: torch.Tensor | None = None   # int32 [slots]
-        self.version = 0                     # of the stacks' addresses
 
     def _fused(self):
         """First projection -> ([(projection, columns)], K) of this TP rank."""
@@ -207,7 +206,7 @@ class LoraBank:
 
     def _stack(self, slot: int, ad: LoraAdapter, device, dtype) -> None:
         """The adapter's matrices into the stacks, which grow where they have
-        no row or rank for them: a growth gives all of them new addresses."""
+        no row or rank for them."""
         fused = self._fused()
         mods: dict[tuple[int, str], dict] = {}
         rank = 0
@@ -248,7 +247,6 @@ class LoraBank:
         for key, g in groups.items():
             g.put(row, mods.get(key, {}))
         self.groups, self.ranks = groups, ranks
-        self.version += bool(new)
         self.slots, self.rank = slots, new_rank
         self.ranks[row:row + 1].fill_(rank)
         if self._free:

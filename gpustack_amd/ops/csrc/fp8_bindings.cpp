@@ -185,13 +185,18 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
   const long T = order.size(0);
   TORCH_CHECK(starts.size(0) == S + 1 && ranks.size(0) == S,
               "lora_add: S + 1 starts and S ranks");
-  TORCH_CHECK(T <= rows && rows < 1l << 31 && S < 1l << 24 && N < 1l << 31 && K < 1l << 31 &&
-              (T + S) / 16 <= 65535 * 8, "lora_add: sizes");
+  TORCH_CHECK(T <= rows && rows < 1l << 31 && S < 1l << 24 && N < 1l << 31 && K < 1l << 31,
+              "lora_add: sizes");
   if (T == 0 || S == 0) return;
   const at::DeviceGuard guard(x.device());
-  // 16 rows a tile below 32 rows a slot on average, 64 below 128, else 128
+  // Tiles of 16 rows up to 767 rows in all, and below 32 a slot, else of 64, from 3072
+  // rows and 192 a slot of 128. us in 16, 64 and 128: 128 rows of one slot, 6144 x 4096,
+  // rank 16, 9.8, 13.7 and 15.6; 32 of each of 16 slots 16.2, 16.1 and 18.1, 64 of each
+  // 21.5, 18.7 and 20.6; 256 of each of 4 slots, 28672 x 4096, 39.6, 35.9 and 37.1; of
+  // each of 16, 4096 x 4096, rank 64, 66, 38.2 and 36.5
   const long used = std::min(S, T), groups = P * ((R + 15) / 16);
-  const LoraPlan plan = lora_plan(T < 32 * used, T >= 128 * used, (int)groups);
+  const LoraPlan plan = lora_plan(T < std::max(768l, 32 * used),
+                                  T >= std::max(3072l, 192 * used), (int)groups);
   // k is cut until the workgroups fill the CUs: of few rows each wave has four units of
   // 64 k then; of many at least four steps are left, and up to five parts, which the
   // second launch reads again for every 512 columns (8192 rows of 4096 x 4096 at rank 64
@@ -203,6 +208,7 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
       : std::min({units / 4, 256 * plan.held / tiles, 5l}));
   // 256 columns of 16 or 32 rows at a time, more in turn where that leaves 1024 workgroups
   const bool few = plan.mt == 1;
+  TORCH_CHECK(lora_tiles(T, S, few ? 16 : 32) <= 65535, "lora_add: sizes");
   const long turns = std::max(1l, std::min(few ? 4l : 2l, lora_tiles(T, S, few ? 16 : 32) *
                                                               ((N + 255) / 256) / 1024));
   Tensor h = at::empty({splits, T, P * R}, x.options().dtype(at::kFloat));

@@ -425,6 +425,10 @@ void lora_launch(void* out, long os, float* h, const void* x, long xs, const voi
                        (unsigned short*)out, os, h, splits, (const unsigned short*)b,
                        order, starts, ranks, rows, T, S, N, R, turns, e);
   };
+  // Of many rows 32 a workgroup, which leave the registers room for more waves (28672
+  // columns at rank 16: 240 us, of 64 rows 307), but 64 where b is as long as what is
+  // read of out (rank 64: 243, of 32 rows 283); at rank 128 their b leaves no room (4096
+  // columns 81, of 32 rows 74).
   if (plan.mt == 1) {
     if (R <= 32) up(lora_up_kernel<1, 1>, 1);
     else if (R <= 64) up(lora_up_kernel<1, 2>, 1);

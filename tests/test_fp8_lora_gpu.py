@@ -178,7 +178,11 @@ ADAPTERS = [  # rows, K, ends, slots, R, kind of batch
     (40, 192, (304,), 3, 256, "steps"), (5, 128, (136,), 200, 128, "steps"),
     (300, 320, (256, 320), 3, 32, "prompts"), (257, 1000, (520,), 2, 72, "prompts"),
     (1000, 136, (96, 192, 392), 7, 16, "prompts"), (511, 512, (640,), 1, 136, "prompts"),
-    (200, 64, (72,), 2, 256, "prompts")]
+    (200, 64, (72,), 2, 256, "prompts"), (2, 8, (8,), 1, 8, "steps"),
+    (900, 72, (64, 200, 264), 4, 64, "prompts"), (800, 200, (88,), 3, 128, "prompts"),
+    (1200, 40, (136, 328), 2, 256, "prompts"), (3300, 168, (72, 144), 2, 24, "prompts"),
+    (3500, 128, (64,), 3, 64, "prompts"), (3100, 96, (32, 64, 96), 1, 48, "prompts"),
+    (3200, 64, (40, 80, 120, 160), 2, 72, "prompts"), (780, 264, (56,), 300, 16, "steps")]
 
 
 def _slots(T, S, kind, seed):
