@@ -18,7 +18,7 @@ void fp8_join_launch(void*, const void*, const float*, const float*, const void*
 void fp8_wide_launch(void*, const void*, const float*, const void*, const float*, const void*, int, int, int, int, int, int, int*, hipStream_t);
 int lora_most_rank();
 LoraPlan lora_plan(bool, bool, int);
-void lora_launch(void*, long, float*, const void*, long, const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, const int*, int, LoraPlan, int, int, hipStream_t);
+void lora_launch(void*, long, float*, const void*, long, const void*, const void*, const int*, const int*, const int*, int, int, int, int, int, int, const int*, int, LoraPlan, int, int, void*, hipStream_t);
 
 #define HIP_CHECK_LAST()                                                     \
   do {                                                                       \
@@ -198,24 +198,32 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
   const LoraPlan plan = lora_plan(T < std::max(768l, 32 * used),
                                   T >= std::max(3072l, 192 * used), (int)groups);
   // k is cut until the workgroups fill the CUs: of few rows each wave has four units of
-  // 64 k then; of many at least four steps are left, and up to five parts, which the
-  // second launch reads again for every 512 columns (8192 rows of 4096 x 4096 at rank 64
-  // in 1, 3 and 7 parts: 38 + 47, 22 + 55 and 23 + 62 us)
+  // 64 k then; of many at least four steps are left, and up to five parts, since the
+  // second launch reads them again for all its columns (8192 rows of 4096 x 4096 at rank
+  // 64 in 1, 3 and 7 parts: 38 + 47, 22 + 55 and 23 + 62 us)
   const long tiles = (long)lora_tiles(T, S, 16 * plan.mt) * ((groups + plan.nt - 1) / plan.nt);
   const long units = (K + 63) / 64;
-  const long splits = std::max(1l, plan.mt == 1
+  const bool few = plan.mt == 1;
+  const long splits = std::max(1l, few
       ? std::min((units + 15) / 16, 4096 / tiles)
       : std::min({units / 4, 256 * plan.held / tiles, 5l}));
-  // 256 columns of 16 or 32 rows at a time, more in turn where that leaves 1024 workgroups
-  const bool few = plan.mt == 1;
-  TORCH_CHECK(lora_tiles(T, S, few ? 16 : 32) <= 65535, "lora_add: sizes");
-  const long turns = std::max(1l, std::min(few ? 4l : 2l, lora_tiles(T, S, few ? 16 : 32) *
-                                                              ((N + 255) / 256) / 1024));
-  Tensor h = at::empty({splits, T, P * R}, x.options().dtype(at::kFloat));
+  // Long ones are added up in a launch of their own (8192 rows of 28672 x 4096 at rank 64
+  // 340 -> 306 us, 1200 of 6144 x 4096 at 128 38.6 -> 36.5; up to rank 32 2039 rows of
+  // 6144 x 4096 26.1 -> 27.6)
+  const bool join = !few && R > 32 && splits > 1;
+  // 256 columns of 16 to 64 rows at a time, more in turn where enough workgroups are left
+  const long up = lora_tiles(T, S, few ? 16 : R > 32 ? 64 : 32), across = (N + 255) / 256;
+  TORCH_CHECK(up <= 65535, "lora_add: sizes");
+  const long turns = std::max(1l, few ? std::min(4l, up * across / 1024)
+                              : R > 32 ? std::min(4l, up * across / 512)
+                                       : std::min(2l, up * across / 512));
+  Tensor h = at::empty({splits, T, P * R}, x.options().dtype(at::kFloat)), joined;
+  if (join) joined = at::empty({2, T, P * R}, x.options());
   lora_launch(out.data_ptr(), os, h.data_ptr<float>(), x.data_ptr(), xs, a.data_ptr(),
               b.data_ptr(), order.data_ptr<int>(), starts.data_ptr<int>(),
               ranks.data_ptr<int>(), (int)rows, (int)T, (int)S, (int)N, (int)K, (int)P, e,
-              (int)R, plan, (int)splits, (int)turns, cur_stream(x));
+              (int)R, plan, (int)splits, (int)turns, join ? joined.data_ptr() : nullptr,
+              cur_stream(x));
   HIP_CHECK_LAST();
 }
 

@@ -7,15 +7,15 @@
 // 16 x 16 x 32 products serve decode steps and prompts alike.
 //
 // Two launches. The first multiplies by a, with k cut over the grid where there are few
-// tiles. Its fp32 sums (h, in `splits` parts) are added up by the second,
-// which holds them as two bf16 parts (the value and what that rounded away, 16 bits of
-// it in all): one would cost h the 2^-9 that the rest of the sum does not lose. Both
-// are bound by memory: x and a, then b and out. us, first and second: one row of 4096 k
-// and 6144 columns in three parts, rank 16, 4.2 and 4.5; 64 rows of 28 adapters, 28672
-// columns in two parts, ranks 1 to 64 of 64, 9 and 27 (of rank 16 in 16, 6 and 9); 2039
-// rows of 8 runs, 6144 columns, rank 32, 15 and 17; 8192 rows, 4096 columns, rank 64, 24
-// and 56, rank 16, 22 and 33; 28672 columns, rank 16, 22 and 200, where adding a number to
-// as many takes 158.
+// tiles. Its fp32 sums (h, in `splits` parts) are added up by the second (of prompts at
+// higher ranks by a launch between the two), which holds them as two bf16 parts (the
+// value and what that rounded away, 16 bits of it in all): one would cost h the 2^-9 that
+// the rest of the sum does not lose. Both are bound by memory: x and a, then b and out.
+// us, first and second: one row of 4096 k and 6144 columns in three parts, rank 16, 4.2
+// and 4.5; 64 rows of 28 adapters, 28672 columns in two parts, ranks 1 to 64 of 64, 9 and
+// 27 (of rank 16 in 16, 6 and 9); 2039 rows of 8 runs, 6144 columns, rank 32, 12 and 14;
+// 8192 rows, 4096 columns, rank 64, 25 and 42 with 4 between, rank 16, 22 and 33; 28672
+// columns, rank 16, 24 and 207, where adding a number to as many takes 158.
 #include "lora.h"
 
 namespace {
@@ -239,6 +239,29 @@ __global__ __launch_bounds__(256) void lora_down_tile_kernel(
   }
 }
 
+// Values as two bf16 parts, the value and what that rounded away (an infinity: nothing).
+DEVICE_INLINE void two_parts(const f32x4& v, u16x4& hi, u16x4& lo) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = f2bf(v[e]);
+    lo[e] = __builtin_isinf(v[e]) ? (unsigned short)0 : f2bf(v[e] - bf2f(hi[e]));
+  }
+}
+
+// The sums of h's parts, [2, n] as two bf16 parts, for a second launch that would
+// otherwise add them up for every workgroup of its rows.
+__global__ __launch_bounds__(256) void lora_join_kernel(
+    unsigned short* __restrict__ to, const float* __restrict__ h, long n, int splits) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 v = *reinterpret_cast<const f32x4*>(h + i);
+  for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(h + s * n + i);
+  u16x4 hi, lo;
+  two_parts(v, hi, lo);
+  *reinterpret_cast<u16x4*>(to + i) = hi;
+  *reinterpret_cast<u16x4*>(to + n + i) = lo;
+}
+
 struct Ends { int n, end[4]; };
 
 // out += h b^T. A workgroup has 16 TT rows and `turns` times 256 columns of one part,
@@ -246,15 +269,17 @@ struct Ends { int n, end[4]; };
 // is 512 neighbouring bytes and more (of 128 rows and 64 columns a workgroup 28672 columns
 // take 236 us for 200): four tiles of 16 weight rows, dealt so that a lane ends
 // with twice 8 neighbours of a row and four lanes with 64 bytes of it. What a turn reads
-// of b and out is asked for before the turn before ends, the first turn's before h. KT:
-// 32 k of the rank at a time that the registers hold (32 KT >= rank).
+// of b and out is asked for before the turn before ends, the first turn's before h (of
+// `joined` h the two parts, [2, T, C]). 32 KT >= rank; of b the registers hold 64 k. Five
+// waves a SIMD of few rows (64 rows of 32 adapters, 28672 columns, rank 64: four 34 us,
+// five 31, six 40).
 template <int TT, int KT>
-__global__ __launch_bounds__(256) void lora_up_kernel(
+__global__ __launch_bounds__(256, TT == 1 && KT <= 2 ? 5 : 1) void lora_up_kernel(
     unsigned short* __restrict__ out, long os, const float* __restrict__ h, int splits,
     const unsigned short* __restrict__ b, const int* __restrict__ order,
     const int* __restrict__ starts, const int* __restrict__ ranks, int rows, int T, int S,
-    int N, int R, int turns, Ends ends) {
-  constexpr int ROWS = 16 * TT, LD = 32 * KT + 8;
+    int N, int R, int turns, bool joined, Ends ends) {
+  constexpr int ROWS = 16 * TT, LD = 32 * KT + 8, KB = KT < 2 ? KT : 2;
   __shared__ __attribute__((aligned(16))) unsigned short part[2][ROWS * LD];
   const Place p = find_tile<ROWS>(blockIdx.y, starts, ranks, S, T, R);
   if (p.count == 0 || p.rank == 0) return;
@@ -284,15 +309,15 @@ __global__ __launch_bounds__(256) void lora_up_kernel(
     const int row = i < p.count ? order[p.first + i] : -1;
     at[t] = row < rows ? row : -1;
   }
-  u32x4 fb[KT][4];
+  u32x4 fb[KB][4];
   u16x8 old[TT][2];
   // row i of tile c is column c / 2 * 32 + i / 4 * 8 + c % 2 * 4 + i % 4
-  auto weights = [&](int n) {
+  auto weights = [&](int n, int k0) {
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
+    for (int k = 0; k < KB; ++k)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int j = k * 32 + lg * 8;
+        const int j = (k0 + k) * 32 + lg * 8;
         const int col = min(n + c / 2 * 32 + (lc >> 2) * 8 + c % 2 * 4 + (lc & 3), high - 1);
         fb[k][c] = *reinterpret_cast<const u32x4*>(
             b + ((long)p.slot * N + col) * R + (j < p.rank ? j : 0));
@@ -308,9 +333,28 @@ __global__ __launch_bounds__(256) void lora_up_kernel(
             out + (at[t] < 0 ? 0 : at[t]) * os + (col < high ? col : low));
       }
   };
-  weights(min(n0, last - 1));
+  weights(min(n0, last - 1), 0);
   before(min(n0, last - 1));
-  for (int i = tid; i < ROWS * 8 * KT; i += 256) {
+  if (TT > 1 && joined)
+    for (int i = tid; i < ROWS * 4 * KT; i += 256) {
+      const int row = i / (4 * KT), j = i % (4 * KT) * 8;
+      u16x8 v[2] = {};
+      if (row < p.count && j < p.rank) {
+        const unsigned short* from = reinterpret_cast<const unsigned short*>(h) +
+                                     (long)(p.first + row) * C + which * R + j;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          v[q] = *reinterpret_cast<const u16x8*>(from + (long)q * T * C);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j + e >= p.rank) v[q][e] = 0;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        *reinterpret_cast<u16x8*>(&part[q][row * LD + j]) = v[q];
+    }
+  else for (int i = tid; i < ROWS * 8 * KT; i += 256) {
     const int row = i / (8 * KT), j = i % (8 * KT) * 4;
     f32x4 v{0.f, 0.f, 0.f, 0.f};
     if (row < p.count && j < p.rank) {
@@ -319,14 +363,11 @@ __global__ __launch_bounds__(256) void lora_up_kernel(
       for (int s = 0; s < splits; ++s)
         v += *reinterpret_cast<const f32x4*>(from + (long)s * T * C);
     }
-    u16x4 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; ++e)
       if (j + e >= p.rank) v[e] = 0.f;
-      hi[e] = f2bf(v[e]);
-      // (an infinity leaves none)
-      lo[e] = __builtin_isinf(v[e]) ? (unsigned short)0 : f2bf(v[e] - bf2f(hi[e]));
-    }
+    u16x4 hi, lo;
+    two_parts(v, hi, lo);
     *reinterpret_cast<u16x4*>(&part[0][row * LD + j]) = hi;
     *reinterpret_cast<u16x4*>(&part[1][row * LD + j]) = lo;
   }
@@ -338,27 +379,32 @@ __global__ __launch_bounds__(256) void lora_up_kernel(
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      if (k * 32 >= p.rank) break;
-      const int j = k * 32 + lg * 8, left = p.rank - j;
-      if (left < 8)                          // what lies behind the rank may be anything
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            fb[k][c][e] &= 2 * e + 1 < left ? ~0u : 2 * e < left ? 0xffffu : 0u;
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(&part[0][(t * 16 + lc) * LD + j]);
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(&part[1][(t * 16 + lc) * LD + j]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          acc[t][c] = multiply(fb[k][c], lo, multiply(fb[k][c], hi, acc[t][c]));
-      }
-    }
     const bool more = n0 + 256 < last;
-    if (more) weights(n0 + 256);
+#pragma unroll
+    for (int k0 = 0; k0 < KT; k0 += KB) {
+      if (k0 > 0 && k0 * 32 >= p.rank) break;
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        if (k > 0 && (k0 + k) * 32 >= p.rank) break;
+        const int j = (k0 + k) * 32 + lg * 8, left = p.rank - j;
+        if (left < 8)                        // what lies behind the rank may be anything
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              fb[k][c][e] &= 2 * e + 1 < left ? ~0u : 2 * e < left ? 0xffffu : 0u;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          const u32x4 hi = *reinterpret_cast<const u32x4*>(&part[0][(t * 16 + lc) * LD + j]);
+          const u32x4 lo = *reinterpret_cast<const u32x4*>(&part[1][(t * 16 + lc) * LD + j]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            acc[t][c] = multiply(fb[k][c], lo, multiply(fb[k][c], hi, acc[t][c]));
+        }
+      }
+      if (k0 + KB < KT && (k0 + KB) * 32 < p.rank) weights(n0, k0 + KB);
+    }
+    if (more) weights(n0 + 256, 0);
     // acc[t][c][r]: row t * 16 + lc, column c / 2 * 32 + lg * 8 + c % 2 * 4 + r; ends are
     // multiples of 8
 #pragma unroll
@@ -389,11 +435,11 @@ LoraPlan lora_plan(bool few, bool many, int groups) {
 }
 
 // rows: of x and out; T: entries of the order. K, R and the ends are multiples of 8.
-// splits: parts of k of h; turns: of 256 columns a workgroup of the second launch.
+// splits: parts of k of h; parts: a place for its sums [2, T, P R], or null; turns: of 256 columns a workgroup of the second launch.
 void lora_launch(void* out, long os, float* h, const void* x, long xs, const void* a,
                  const void* b, const int* order, const int* starts, const int* ranks,
                  int rows, int T, int S, int N, int K, int P, const int* ends, int R,
-                 LoraPlan plan, int splits, int turns, hipStream_t s) {
+                 LoraPlan plan, int splits, int turns, void* parts, hipStream_t s) {
   const int groups = P * ((R + 15) / 16);
   auto down = [&](auto kernel) {
     hipLaunchKernelGGL(kernel,
@@ -413,6 +459,11 @@ void lora_launch(void* out, long os, float* h, const void* x, long xs, const voi
     case 808: down(lora_down_tile_kernel<8, 8, 4>); break;
     case 812: down(lora_down_tile_kernel<8, 12, 4>); break;
   }
+  if (parts) {
+    const long n = (long)T * P * R;
+    hipLaunchKernelGGL(lora_join_kernel, dim3((n / 4 + 255) / 256), dim3(256), 0, s,
+                       (unsigned short*)parts, h, n, splits);
+  }
   Ends e{P, {0, 0, 0, 0}};
   const int wide = 256 * turns;
   int blocks = 0;
@@ -422,13 +473,13 @@ void lora_launch(void* out, long os, float* h, const void* x, long xs, const voi
   }
   auto up = [&](auto kernel, int tt) {
     hipLaunchKernelGGL(kernel, dim3(blocks, lora_tiles(T, S, 16 * tt)), dim3(256), 0, s,
-                       (unsigned short*)out, os, h, splits, (const unsigned short*)b,
-                       order, starts, ranks, rows, T, S, N, R, turns, e);
+                       (unsigned short*)out, os, parts ? (const float*)parts : h, splits,
+                       (const unsigned short*)b, order, starts, ranks, rows, T, S, N, R,
+                       turns, parts != nullptr, e);
   };
   // Of many rows 32 a workgroup, which leave the registers room for more waves (28672
   // columns at rank 16: 240 us, of 64 rows 307), but 64 where b is as long as what is
-  // read of out (rank 64: 243, of 32 rows 283); at rank 128 their b leaves no room (4096
-  // columns 81, of 32 rows 74).
+  // read of out (rank 64: 243, of 32 rows 283).
   if (plan.mt == 1) {
     if (R <= 32) up(lora_up_kernel<1, 1>, 1);
     else if (R <= 64) up(lora_up_kernel<1, 2>, 1);
@@ -437,7 +488,7 @@ void lora_launch(void* out, long os, float* h, const void* x, long xs, const voi
   } else {
     if (R <= 32) up(lora_up_kernel<2, 1>, 2);
     else if (R <= 64) up(lora_up_kernel<4, 2>, 4);
-    else if (R <= 128) up(lora_up_kernel<2, 4>, 2);
-    else up(lora_up_kernel<2, 8>, 2);
+    else if (R <= 128) up(lora_up_kernel<4, 4>, 4);
+    else up(lora_up_kernel<4, 8>, 4);
   }
 }
