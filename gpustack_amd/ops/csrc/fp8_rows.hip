@@ -10,9 +10,16 @@
 // they are above every number, so its scale is the infinity or NaN and so are its
 // products.
 //
-// Bound by memory: each row is read once and held in registers between its sums, its
-// maximum and its rounding. A row takes a wave up to 1024 channels (four rows a
-// workgroup), 256 threads up to 8192, 1024 beyond.
+// Rounded once means: of x, and of r w, the quotients are those of exact numbers, so
+// that values halfway between two of e4m3, which bf16 rows have, go to the even one; of
+// silu, which is an fp32 value itself, about one in two million goes to another
+// one than in 64 bits.
+//
+// Bound by memory: each row is read once and held in registers; its squares and its
+// largest value are summed up in one exchange. A row takes a wave up to 1024 channels
+// (four rows a workgroup), 256 threads up to 8192, 1024 beyond. 8192 rows of 5120 with
+// the residual 51 us (5.8 TB/s), and in bf16 too 71 (5.3), of 4096 37 and 48 (6.3); silu
+// of 8192 x 4096 34 (4.9), 512 x 8192 7.2; 64 rows of 14336 5.4, launch and latency.
 #include "common.h"
 
 namespace {
@@ -49,9 +56,13 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
   if (G < 256 && row >= T) return;           // whole waves; none waits for another
   const unsigned short* xr = x + row * xs;
 
+  // the row: v, but of the norm r, whose products with the weights are exact
   float v[NV][8];
+  u16x8 wv[SRC == NORM ? NV : 1];
+  auto value = [&](int i, int j) {
+    return SRC == NORM ? v[i][j] * bf2f(wv[i][j]) : v[i][j];
+  };
   float squares = 0.f;
-  unsigned top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * G + t) * 8;
@@ -65,6 +76,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
         if (rows) *reinterpret_cast<u16x8*>(rows + row * H + c) = f32_to_bf8(v[i]);
       } else {
         u16x8 r = a;
+        if constexpr (SRC == NORM) wv[i] = *reinterpret_cast<const u16x8*>(weight + c);
         if (SRC == NORM && residual) {
           const u16x8 b = *reinterpret_cast<const u16x8*>(residual + row * H + c);
 #pragma unroll
@@ -79,51 +91,64 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      if constexpr (SRC == NORM) wv[i] = u16x8{};
     }
   }
-  if constexpr (SRC == NORM) {
-    squares = wave_reduce_sum(squares);
+  // the largest value of the row, and its squares' sum
+  auto largest = [&](auto of) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        top = max(top, __builtin_bit_cast(unsigned, of(i, j)) & 0x7fffffffu);
+    top = wave_max_bits(top);
+    if constexpr (SRC == NORM) squares = wave_reduce_sum(squares);
     if constexpr (WAVES > 1) {
-      if (t % WAVE_SIZE == 0) part[0][t / WAVE_SIZE] = squares;
+      if (t % WAVE_SIZE == 0) {
+        part[0][t / WAVE_SIZE] = __builtin_bit_cast(float, top);
+        if constexpr (SRC == NORM) part[1][t / WAVE_SIZE] = squares;
+      }
       __syncthreads();
       squares = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) squares += part[0][w];
-    }
-    const float inv = 1.f / sqrtf(squares / (float)H + eps);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + t) * 8;
-      if (c < H) {
-        const u16x8 w = *reinterpret_cast<const u16x8*>(weight + c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * bf2f(w[j]);
-        if (rows) *reinterpret_cast<u16x8*>(rows + row * H + c) = f32_to_bf8(v[i]);
+      for (int w = 0; w < WAVES; ++w) {
+        top = max(top, __builtin_bit_cast(unsigned, part[0][w]));
+        if constexpr (SRC == NORM) squares += part[1][w];
       }
     }
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      top = max(top, __builtin_bit_cast(unsigned, v[i][j]) & 0x7fffffffu);
-  top = wave_max_bits(top);
-  if constexpr (WAVES > 1) {
-    if (t % WAVE_SIZE == 0) part[1][t / WAVE_SIZE] = __builtin_bit_cast(float, top);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w)
-      top = max(top, __builtin_bit_cast(unsigned, part[1][w]));
-  }
-  const float most = __builtin_bit_cast(float, top);
+    return __builtin_bit_cast(float, top);
+  };
+  float most = largest(value), inv = 1.f;
+  if constexpr (SRC == NORM) inv = 1.f / sqrtf(squares / (float)H + eps);
   // a NaN is neither below nor above the least scale, and stays
-  const float s = most / TOP < LEAST ? LEAST : most / TOP;
+  float s = most * inv / TOP;
+  // v / s = 448 a / max(|a|) of the values a = r w or x, which are exact, as is 448 a: one
+  // rounding, and none of values between two of e4m3, which go to the even one
+  float over = most, times = TOP;
+  if (SRC == SILU || !(most > 0x1p-60f && most < 0x1p100f && s >= LEAST)) {
+    if constexpr (SRC == NORM) {              // r w may have left fp32 where v has not
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[i][j] = v[i][j] * inv * bf2f(wv[i][j]);
+          wv[i][j] = 0x3f80;                  // one
+        }
+      if constexpr (WAVES > 1) __syncthreads();
+      most = largest(value);
+      inv = 1.f;
+    }
+    s = most / TOP < LEAST ? LEAST : most / TOP;
+    over = s;
+    times = 1.f;
+  }
   // the quotients as a division rounds them: by the reciprocal, put right by what that
   // leaves, of finite scales
-  const float turn = 1.f / s, left = s < INFINITY ? turn : 0.f;
-  auto over = [&](float a) {
-    const float r = a * turn;
-    return left == 0.f ? r : __builtin_fmaf(__builtin_fmaf(-r, s, a), left, r);
+  const float turn = 1.f / over, left = over < INFINITY ? turn : 0.f;
+  auto quotient = [&](int i, int j) {
+    const float a = value(i, j) * times, r = a * turn;
+    return left == 0.f ? r : __builtin_fmaf(__builtin_fmaf(-r, over, a), left, r);
   };
   if (t == 0) scale[row] = s;
 #pragma unroll
@@ -132,12 +157,18 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
     if (c < H) {
       uint2 o;
       int lo = 0, hi = 0;
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][0]), over(v[i][1]), lo, false);
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][2]), over(v[i][3]), lo, true);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][4]), over(v[i][5]), hi, false);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(over(v[i][6]), over(v[i][7]), hi, true);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 0), quotient(i, 1), lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 2), quotient(i, 3), lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 4), quotient(i, 5), hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 6), quotient(i, 7), hi, true);
       o.x = lo;
       o.y = hi;
+      if (SRC == NORM && rows) {
+        float u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = value(i, j) * inv;
+        *reinterpret_cast<u16x8*>(rows + row * H + c) = f32_to_bf8(u);
+      }
       *reinterpret_cast<uint2*>(q + row * H + c) = o;
     }
   }
