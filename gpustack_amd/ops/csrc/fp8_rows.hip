@@ -11,12 +11,12 @@
 // products.
 //
 // Rounded once means: of x, and of r w, the quotients are those of exact numbers, so
-// that values halfway between two of e4m3, which bf16 rows have, go to the even one; of
-// silu, which is an fp32 value itself, about one in two million goes to another
-// one than in 64 bits.
+// that values halfway between two of e4m3, which bf16 rows have, go to the even one. Of
+// silu, which is an fp32 value itself, about one in two million goes to another one than
+// in 64 bits.
 //
-// Bound by memory: each row is read once and held in registers; its squares and its
-// largest value are summed up in one exchange. A row takes a wave up to 1024 channels
+// Bound by memory: each row is read once and held in registers; the sum of its squares and
+// its largest value take one exchange. A row takes a wave up to 1024 channels
 // (four rows a workgroup), 256 threads up to 8192, 1024 beyond. 8192 rows of 5120 with
 // the residual 51 us (5.8 TB/s), and in bf16 too 71 (5.3), of 4096 37 and 48 (6.3); silu
 // of 8192 x 4096 34 (4.9), 512 x 8192 7.2; 64 rows of 14336 5.4, launch and latency.

@@ -70,6 +70,36 @@ def test_norm(width, rows, keep, residual):
         assert ((r.rows.double() - v).abs() <= v.abs() * (2 ** -8 + 2 * slack)).all()
 
 
+def test_halfway_values_go_to_the_even_one():
+    """Of bf16 rows 448 v / max(|v|) is exact in 64 bits where it lies halfway
+    between two e4m3 values, as it often does."""
+    x = _randn(64, 4096, seed=8).cuda()
+    d = x.double()
+    want = (d * 448 / d.abs().amax(1, keepdim=True)).to(E4M3)
+    assert torch.equal(ops.rows_fp8(x).q.float(), want.float())
+    w = _randn(4096, seed=9).cuda()
+    p = d * w.double()
+    want = (p * 448 / p.abs().amax(1, keepdim=True)).to(E4M3)
+    r, _ = ops.add_rms_norm_fp8(x, None, w, 1e-5)
+    assert torch.equal(r.q.float(), want.float())
+
+
+@pytest.mark.parametrize("width", [512, 4096, 16384])
+@pytest.mark.parametrize("size,weight", [(1e10, 1e30), (1e-15, 1e-12), (1e15, 1e-30),
+                                         (1e-25, 1e20)])
+def test_norm_whose_products_leave_fp32(width, size, weight):
+    """r w may be beyond fp32, or below it, where v is not; rows below the least
+    scale are held in its steps."""
+    x = (_randn(3, width, seed=1).float() * size).bfloat16().cuda()
+    w = (_randn(width, seed=2).float() * weight).bfloat16().cuda()
+    r, _ = ops.add_rms_norm_fp8(x, None, w, 1e-5, rows=True)
+    t = x.double()
+    v = t * (t.square().mean(1, keepdim=True) + 1e-5) ** -.5 * w.double()
+    _check_rows(r, v, 100 * 2. ** -24)
+    # values below fp32's least normal one may be lost
+    assert ((r.rows.double() - v).abs() <= v.abs() * (2 ** -8 + 2 ** -16) + 2. ** -126).all()
+
+
 def test_rows_of_a_slice_and_without_numbers():
     base = _randn(9, 4096, seed=5).cuda()
     x = base[1::2, 1024:1544]                  # rows of 520 of stride 8192
