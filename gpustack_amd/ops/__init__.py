@@ -2031,35 +2031,36 @@ def add_rms_norm_fp8(x, residual, weight, eps: float, rows: bool = False):
 # (fp8_rows_gemm_kernel), 16 rows and columns of a tile (fp8_tile_kernel), 32 of them
 # (fp8_wide_kernel): the launch, a round, a round's step, a step's share of all the
 # steps over the CUs, a MB of weights, a join, a MB of its parts (of the first: a round's
-# step and row), a MB of the result. Fitted to 8126 sizes (1 to 8192 rows, 512 to 28672
-# columns, 512 to 15360 k, weights out of HBM), off by 5 to 10 % of a time; the least by
-# them costs 2 % more than the best on average, 5 % in one size of six.
+# step and row), a MB of the result. Fitted to 9665 sizes (1 to 8192 rows, 512 to 28672
+# columns, 512 to 15344 k, weights out of HBM), off by 6 to 13 % of a time (those of the
+# first 13 to 18 %); the least by them costs 3 % more than the best on average, 5 % in one
+# size of five.
 _FP8_ROWS = {
-    (1, 16): (2.27, .351, .798, 0, .164, .037, 1.00, .01),
-    (1, 32): (2.09, .174, 1.71, .177, .173, .034, 4.04, .711),
-    (2, 16): (1.89, .601, .656, 0, .168, .05, 1.00, 0),
-    (2, 32): (1.61, .924, 1.51, .074, .181, .052, 1.76, .339),
-    (4, 16): (1.79, .999, 1.43, 0, .285, .034, 1.00, .202)}
+    (1, 16): (3.02, .39, .492, 0, .166, .031, 1.00, .001),
+    (1, 32): (2.47, .346, 1.44, 0, .174, .03, 1.00, .011),
+    (2, 16): (2.25, .877, .337, 0, .169, .042, 1.00, 0),
+    (2, 32): (1.65, .941, 1.53, .267, .197, .036, 1.00, 0),
+    (4, 16): (1.73, 1.13, .939, 0, .285, .032, 1.00, 0)}
 _FP8_TILES = {
-    (2, 2): (1.25, 1.63, .158, .045, .181, 3.47, 1.33, 0),
-    (2, 4): (1.58, 1.27, .118, .13, .173, 3.34, 1.03, 0),
-    (2, 8): (2.26, 1.13, 0, .372, .172, 2.52, 1.13, .05),
-    (4, 2): (2.31, .298, .256, .019, .215, 2.85, 1.63, .148),
-    (4, 4): (2.82, .344, .217, .122, .157, 2.33, 1.44, .077),
-    (4, 8): (4.04, 0, .039, .424, .138, 1.43, 1.51, .024),
-    (8, 2): (2.60, .441, .295, .104, .283, 2.15, 1.60, .198),
-    (8, 4): (4.01, 0, .144, .316, .188, 1.36, 1.57, .185),
-    (8, 8): (5.73, .178, .415, .215, .157, 0, 1.49, .202)}
+    (2, 2): (.997, 2.52, .148, .039, .201, 3.40, 1.70, 0),
+    (2, 4): (2.04, 1.22, .09, .146, .178, 3.40, .855, 0),
+    (2, 8): (2.37, 1.19, 0, .376, .184, 2.73, 1.13, .041),
+    (4, 2): (2.19, 1.05, .224, .021, .251, 3.16, 1.11, 0),
+    (4, 4): (2.70, .671, .121, .2, .18, 2.79, 1.16, 0),
+    (4, 8): (4.08, .001, .05, .42, .157, 1.74, 1.40, 0),
+    (8, 2): (2.64, .599, .237, .154, .318, 2.53, 1.34, .121),
+    (8, 4): (4.26, 0, .183, .275, .205, 1.50, 1.48, .054),
+    (8, 8): (5.93, 0, .421, .221, .17, 0, 1.59, .156)}
 _FP8_WIDE = {
-    (4, 2): (3.12, .798, .255, .064, .247, 2.40, 2.10, .072),
-    (4, 4): (3.56, .925, .346, .134, .209, 2.69, 1.84, .1),
-    (4, 6): (4.05, .828, .464, .176, .184, 3.14, 1.58, .139),
-    (4, 8): (4.44, .519, .57, .25, .182, 3.54, 1.40, .151),
-    (6, 6): (3.56, 1.71, .606, .19, .166, 3.52, 1.40, .15),
-    (6, 8): (3.29, 2.67, .757, .225, .175, 4.01, 1.25, .151),
-    (8, 4): (4.18, .954, .546, .192, .147, 3.02, 1.58, .189),
-    (8, 6): (3.48, 2.51, .734, .221, .126, 3.59, 1.29, .184),
-    (8, 8): (3.18, 3.82, .928, .234, .159, 3.86, 1.22, .174)}
+    (4, 2): (3.34, .496, .299, .063, .282, 2.49, 2.13, .122),
+    (4, 4): (3.83, .407, .417, .126, .224, 2.77, 1.95, .135),
+    (4, 6): (4.50, .142, .557, .147, .212, 3.02, 1.68, .174),
+    (4, 8): (4.53, 0, .696, .198, .213, 3.50, 1.44, .168),
+    (6, 6): (4.04, 1.17, .652, .235, .195, 3.56, 1.45, .148),
+    (6, 8): (3.79, 2.11, .808, .278, .204, 3.91, 1.26, .142),
+    (8, 4): (4.47, .602, .589, .228, .156, 2.95, 1.66, .178),
+    (8, 6): (3.67, 2.35, .77, .295, .162, 3.67, 1.30, .165),
+    (8, 8): (3.58, 3.51, .972, .322, .187, 3.95, 1.20, .162)}
 # workgroups of a tile that a CU holds
 _FP8_HELD = {(2, 2): 5, (2, 4): 3, (2, 8): 2, (4, 2): 3, (4, 4): 2, (4, 8): 2,
              (8, 2): 2, (8, 4): 2, (8, 8): 1}

@@ -24,7 +24,11 @@ DEVICE_INLINE f32x4 multiply(const Bytes32& a, const Bytes32& b, const f32x4& c)
 
 // Up to 16 MT rows. A workgroup of 8 waves owns 16 NTW columns; its waves take the
 // blocks of 256 k of those weight rows in turn, straight from memory, one block ahead
-// with the rows', and meet in the LDS at the end. x comes from the L2. TAIL: the last block is not whole.
+// with the rows', and meet in the LDS at the end. x comes from the L2, which bounds more
+// than a few rows: every workgroup reads them all, so from about 32 the tiles below take
+// over. TAIL: the last block is not whole.
+// Bound by the weights out of HBM: one row of 6144 x 4096 7.3 us (3.4 TB/s; by tiles
+// 9.1), 32 rows of 4096 x 4096 7.9 (8.3).
 constexpr int FR_K = 256, FR_WAVES = 8, FR_THREADS = FR_WAVES * WAVE_SIZE;
 
 template <int MT, int NTW, bool TAIL>
@@ -135,7 +139,11 @@ __global__ __launch_bounds__(FR_THREADS) void fp8_rows_gemm_kernel(
 // of 128 k go to a ring of S buffers in the LDS, S - 1 steps ahead of the products. Rows
 // of 128 bytes, the 16-byte piece c of row r at c ^ (r / 2 % 8), which 16 rows read
 // without conflict. Pieces behind the end of a row come from zeros. Few columns are cut
-// over k into fp32 parts that fp8_join_kernel adds up.
+// over k into fp32 parts that fp8_join_kernel adds up: a launch more, and the parts'
+// way through the L2, for the CUs that had none.
+// Bound by the weights out of HBM and by how far ahead they are asked for: 61 rows of
+// 28672 x 4096 26 us whole (4.5 TB/s) in tiles of 64 x 128, 29.7 in two parts; 64 rows of
+// 4096 x 14336 17 us in four parts of 64 x 64 (3.5 TB/s).
 constexpr int FT_K = 128;
 
 __device__ const u32x4 fp8_zeros = {0, 0, 0, 0};

@@ -54,6 +54,31 @@ def test_norm_is_the_unfused_one(rows):
     assert same is total and torch.equal(alone.q.float(), r.q.float())
 
 
+def test_product_plans_are_the_kernels():
+    r = np.random.default_rng(5)
+    sizes = [(1, 8, 16), (64, 8, 16), (65, 8, 16), (300, 8, 112), (301, 16, 112),
+             (65, 8, 128), (8192, 128256, 16384), (65, 2 ** 21, 1040),
+             (100000, 64, 96), (1, 8, 2 ** 22), (70, 64, 2 ** 22)]
+    for _ in range(300):
+        sizes.append((int(2 ** r.uniform(0, 14)), 8 * int(2 ** r.uniform(0, 13)),
+                      16 * int(2 ** r.uniform(0, 11))))
+    for M, N, K in sizes:
+        kind, a, b, splits = ops._fp8_plan(M, N, K)
+        assert 1 <= splits <= min(64, -(-K // 128)), (M, N, K)
+        if kind == 0:
+            assert (a, b) in {(1, 16), (1, 32), (2, 16), (2, 32), (4, 16)}
+            assert M <= 16 * a and splits == 1
+        elif kind == 1:
+            assert a in (2, 4, 8) and b in (2, 4, 8) and M <= 65535 * 16 * a
+        else:
+            assert (a, b) in {(8, 8), (8, 6), (8, 4), (6, 8), (6, 6), (4, 8), (4, 6),
+                              (4, 4), (4, 2)}
+            assert splits <= (-(-K // 128) + 1) // 2 and K >= 128
+            # 32 bits of an operand's offsets and of a tile of the result's
+            assert (N + 256) * K < 2 ** (31 if K % 128 else 32)
+            assert 4 * N * 257 < 2 ** 32 - 256
+
+
 def test_batch_lists():
     order, starts = ops.build_lora_rows([2, -1, 0, 2, 7, 0], 3, "cpu")
     assert order.dtype == starts.dtype == torch.int32
