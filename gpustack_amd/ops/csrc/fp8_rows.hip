@@ -12,14 +12,14 @@
 //
 // Rounded once means: of x, and of r w, the quotients are those of exact numbers, so
 // that values halfway between two of e4m3, which bf16 rows have, go to the even one. Of
-// silu, which is an fp32 value itself, about one in two million goes to another one than
-// in 64 bits.
+// silu, whose fp32 values leave open where one in 60000 belongs, 64 bits decide for those.
 //
 // Bound by memory: each row is read once and held in registers; the sum of its squares and
 // its largest value take one exchange. A row takes a wave up to 1024 channels
 // (four rows a workgroup), 256 threads up to 8192, 1024 beyond. 8192 rows of 5120 with
-// the residual 51 us (5.8 TB/s), and in bf16 too 71 (5.3), of 4096 37 and 48 (6.3); silu
-// of 8192 x 4096 34 (4.9), 512 x 8192 7.2; 64 rows of 14336 5.4, launch and latency.
+// the residual 51 us (5.7 TB/s), and in bf16 too 71 (5.3), of 4096 38 and 49 (6.2); silu
+// of 8192 x 4096 41 (4.1; 36 without the 64 bits, whose waves hold up a workgroup's
+// others), 509 x 14336 12.9 (11.4); 64 rows of 14336 5.5, silu 6.5, launch and latency.
 #include "common.h"
 
 namespace {
@@ -40,20 +40,20 @@ DEVICE_INLINE unsigned wave_max_bits(unsigned v) {
   return max(v, u(row_turned<1>(f(v))));
 }
 
-// G threads a row, NV times 8 values each; 256 / G rows a workgroup below 256.
+// G threads a row, NV times 8 values each; a wave's rows by four a workgroup.
 template <int SRC, int G, int NV>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
+__global__ __launch_bounds__(G == WAVE_SIZE ? 256 : G) void fp8_rows_kernel(
     unsigned char* __restrict__ q, float* __restrict__ scale,
     unsigned short* __restrict__ sum,        // NORM: x + residual, with a residual
     unsigned short* __restrict__ rows,       // NORM, SILU: v in bf16, or null
     const unsigned short* __restrict__ x, long xs,
     const unsigned short* __restrict__ residual,
     const unsigned short* __restrict__ weight, float eps, int T, int H) {
-  constexpr int ROWS = G < 256 ? 256 / G : 1, WAVES = G / WAVE_SIZE;
+  constexpr int ROWS = G == WAVE_SIZE ? 4 : 1, WAVES = G / WAVE_SIZE;
   __shared__ float part[2][WAVES];
   const int t = threadIdx.x % G;
   const long row = (long)blockIdx.x * ROWS + threadIdx.x / G;
-  if (G < 256 && row >= T) return;           // whole waves; none waits for another
+  if (row >= T) return;                      // whole waves; none waits for another
   const unsigned short* xr = x + row * xs;
 
   // the row: v, but of the norm r, whose products with the weights are exact
@@ -94,20 +94,35 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
       if constexpr (SRC == NORM) wv[i] = u16x8{};
     }
   }
-  // the largest value of the row, and its squares' sum
+  // the largest value of the row, and the sum of the squares, or of silu the channel of
+  // this wave's largest
+  int where = 0;
   auto largest = [&](auto of) {
     unsigned top = 0;
+    auto size = [&](int i, int j) {
+      return __builtin_bit_cast(unsigned, of(i, j)) & 0x7fffffffu;
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        top = max(top, __builtin_bit_cast(unsigned, of(i, j)) & 0x7fffffffu);
+      for (int j = 0; j < 8; ++j) top = max(top, size(i, j));
+    const unsigned own = top;
     top = wave_max_bits(top);
     if constexpr (SRC == NORM) squares = wave_reduce_sum(squares);
+    if constexpr (SRC == SILU) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          where = size(i, j) == top ? (i * G + t) * 8 + j : where;
+      where = __builtin_amdgcn_readlane(where, __builtin_ctzll(__ballot(own == top)));
+    }
     if constexpr (WAVES > 1) {
       if (t % WAVE_SIZE == 0) {
         part[0][t / WAVE_SIZE] = __builtin_bit_cast(float, top);
         if constexpr (SRC == NORM) part[1][t / WAVE_SIZE] = squares;
+        if constexpr (SRC == SILU)
+          part[1][t / WAVE_SIZE] = __builtin_bit_cast(float, where);
       }
       __syncthreads();
       squares = 0.f;
@@ -151,16 +166,46 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
     return left == 0.f ? r : __builtin_fmaf(__builtin_fmaf(-r, over, a), left, r);
   };
   if (t == 0) scale[row] = s;
+  unsigned long long left_open = 0;
+
+  // 448 v / max(|v|) of channel c from 64 bits, of rows that are not all zeros
+  auto settled = [&](int c) {
+    const double g = bf2f(xr[c]), u = bf2f(xr[H + c]);
+    if constexpr (WAVES > 1)
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        if (part[0][w] == most) where = __builtin_bit_cast(int, part[1][w]);
+    const double g0 = bf2f(xr[where]), u0 = bf2f(xr[H + where]);
+    const double top = fabs(g0 * u0), below = (1. + exp(-g0)) * TOP;
+    const bool least = top < LEAST * below;
+    return (float)(g * u * (least ? 1. : below) /
+                   ((1. + exp(-g)) * (least ? (double)LEAST : top)));
+  };
+  // fp32 quotients of fp32 silus are off by up to 8.5 2^-24 (3.25 each of the value and
+  // of the largest, two divisions), at most as many steps: within 9 of a value between two
+  // of e4m3 they may be on its other side. (Below 2^-6, whose steps e4m3 keeps, 2^-6 more
+  // has them, too.)
+  auto open = [&](float r) {
+    const float a = __builtin_fabsf(r), b = a < 0x1p-6f ? a + 0x1p-6f : a;
+    return ((__builtin_bit_cast(unsigned, b) & 0xfffffu) - (0x80000u - 9u)) <= 18u &&
+           s < INFINITY;
+  };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * G + t) * 8;
     if (c < H) {
       uint2 o;
       int lo = 0, hi = 0;
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 0), quotient(i, 1), lo, false);
-      lo = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 2), quotient(i, 3), lo, true);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 4), quotient(i, 5), hi, false);
-      hi = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(i, 6), quotient(i, 7), hi, true);
+      float r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = quotient(i, j);
+      if constexpr (SRC == SILU)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) left_open |= open(r[j]) ? 1ull << (i * 8 + j) : 0ull;
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(r[4], r[5], hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(r[6], r[7], hi, true);
       o.x = lo;
       o.y = hi;
       if (SRC == NORM && rows) {
@@ -172,6 +217,14 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void fp8_rows_kernel(
       *reinterpret_cast<uint2*>(q + row * H + c) = o;
     }
   }
+  // written over, by the same lane: the row is in no registers by now
+  if constexpr (SRC == SILU)
+    while (left_open) {
+      const int k = __builtin_ctzll(left_open), c = (k / 8 * G + t) * 8 + k % 8;
+      left_open &= left_open - 1;
+      const float f = settled(c);
+      q[row * H + c] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false);
+    }
 }
 
 }  // namespace
@@ -183,16 +236,23 @@ void fp8_rows_launch(int source, void* q, float* scale, void* sum, void* rows,
                      const void* x, long xs, const void* residual, const void* weight,
                      float eps, int T, int H, hipStream_t s) {
   auto go = [&](auto kernel, int g) {
-    const int each = g < 256 ? 256 / g : 1;
-    hipLaunchKernelGGL(kernel, dim3((T + each - 1) / each), dim3(g < 256 ? 256 : g), 0, s,
+    const bool wave = g == WAVE_SIZE;
+    hipLaunchKernelGGL(kernel, dim3(wave ? (T + 3) / 4 : T), dim3(wave ? 256 : g), 0, s,
                        (unsigned char*)q, scale, (unsigned short*)sum,
                        (unsigned short*)rows, (const unsigned short*)x, xs,
                        (const unsigned short*)residual, (const unsigned short*)weight,
                        eps, T, H);
   };
+  // Rows that leave CUs idle take as many threads as have 8 values of them. us in a
+  // captured graph, norm of 5120 channels: one row 3.38 -> 2.91, 256 4.22 -> 3.78; but
+  // 512 5.44 -> 5.59, 1024 7.75 -> 9.13.
+  const bool few = T <= 256;
   auto by_size = [&](auto src) {
     constexpr int SRC = decltype(src)::value;
-    if (H <= 512) go(fp8_rows_kernel<SRC, 64, 1>, 64);
+    if (few && H > 512 && H <= 1024) go(fp8_rows_kernel<SRC, 128, 1>, 128);
+    else if (few && H > 2048 && H <= 4096) go(fp8_rows_kernel<SRC, 512, 1>, 512);
+    else if (few && H > 4096 && H <= 8192) go(fp8_rows_kernel<SRC, 1024, 1>, 1024);
+    else if (H <= 512) go(fp8_rows_kernel<SRC, 64, 1>, 64);
     else if (H <= 1024) go(fp8_rows_kernel<SRC, 64, 2>, 64);
     else if (H <= 2048) go(fp8_rows_kernel<SRC, 256, 1>, 256);
     else if (H <= 4096) go(fp8_rows_kernel<SRC, 256, 2>, 256);

@@ -84,6 +84,17 @@ def test_halfway_values_go_to_the_even_one():
     assert torch.equal(r.q.float(), want.float())
 
 
+@pytest.mark.parametrize("rows,width", [(1, 520), (700, 1024), (256, 4096), (300, 8192),
+                                        (64, 14336)])
+def test_silu_goes_to_the_nearest_value(rows, width):
+    """Those that 64 bits give, where fp32 would leave some open."""
+    x = (2 * _randn(rows, 2 * width, seed=11)).bfloat16().cuda()
+    g, u = x.double().chunk(2, 1)
+    v = g / (1 + torch.exp(-g)) * u
+    want = (v * 448 / v.abs().amax(1, keepdim=True)).to(E4M3)
+    assert torch.equal(ops.silu_and_mul_fp8(x).q.float(), want.float())
+
+
 @pytest.mark.parametrize("width", [512, 4096, 16384])
 @pytest.mark.parametrize("size,weight", [(1e10, 1e30), (1e-15, 1e-12), (1e15, 1e-30),
                                          (1e-25, 1e20)])
