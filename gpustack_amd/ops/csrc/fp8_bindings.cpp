@@ -198,15 +198,19 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
   const LoraPlan plan = lora_plan(T < std::max(768l, 32 * used),
                                   T >= std::max(3072l, 192 * used), (int)groups);
   // k is cut until the workgroups fill the CUs: of few rows each wave has four units of
-  // 64 k then; of many at least four steps are left, and up to five parts, since the
-  // second launch reads them again for all its columns (8192 rows of 4096 x 4096 at rank
-  // 64 in 1, 3 and 7 parts: 38 + 47, 22 + 55 and 23 + 62 us)
+  // 64 k then; of many at least four steps are left, and up to five parts where the second
+  // launch adds them up, 16 where one of their own does. One workgroup a CU: what a second
+  // gains costs more as a part (us with as many as a CU holds -> one: 8192 rows of 4096 x
+  // 4096 at rank 64 75.9 -> 71.6, at 16 49.5 -> 45.0; 1272 of 19972 x 10672 at 48 71 -> 64),
+  // but where the second launch has few columns to read them for (5366 rows of
+  // 456 x 14320 at 32 44.3 -> 48.7)
   const long tiles = (long)lora_tiles(T, S, 16 * plan.mt) * ((groups + plan.nt - 1) / plan.nt);
   const long units = (K + 63) / 64;
   const bool few = plan.mt == 1;
   const long splits = std::max(1l, few
       ? std::min((units + 15) / 16, 4096 / tiles)
-      : std::min({units / 4, 256 * plan.held / tiles, 5l}));
+      : std::min({units / 4, 256 * (R <= 32 && N <= 1024 ? plan.held : 1) / tiles,
+                  R > 32 ? 16l : 5l}));
   // Long ones are added up in a launch of their own (8192 rows of 28672 x 4096 at rank 64
   // 340 -> 306 us, 1200 of 6144 x 4096 at 128 38.6 -> 36.5; up to rank 32 2039 rows of
   // 6144 x 4096 26.1 -> 27.6)
