@@ -19,11 +19,12 @@
 // Steps come in pairs; an odd number gets one of zeros. Of a step that reaches behind
 // the end of the rows, those pieces are loaded from beyond the operands: zeros, too.
 //
-// Bound by the matrix unit's power: 8192 rows of 28672 x 4096 724 us (2.66 PFLOP/s; in
-// tiles of 256 x 256 777, their last round being short), 8192 of 4096 x 14336 296 (3.25),
-// 4097 of the same 176 (2.73, in 192 x 192). By its rounds where they leave CUs idle:
+// Bound by the matrix unit's power: 8192 rows of 28672 x 4096 723 us (2.66 PFLOP/s; in
+// tiles of 192 x 256 740, of 192 x 192 820), 8192 of 4096 x 14336 316 (3.04; 352 and 387),
+// 4097 of the same 176 in 192 x 192 (2.73; in 256 x 256, whose 272 tiles are a round and a
+// sixteenth, 259). By the rounds where they leave CUs idle:
 // 2039 rows of 6144 x 4096 41 us (2.48 PFLOP/s, 192 tiles of 256 x 192 at once), 523 of
-// 4096 x 14336 45 (1.37, 240 workgroups on five parts, a quarter of it their join).
+// 4096 x 14336 43 (1.43, 240 workgroups on five parts, a fifth of it their join).
 #include "wide_tiles.h"
 
 namespace {
