@@ -2111,7 +2111,7 @@ def _fp8_plan(M: int, N: int, K: int):
     if wide:
         for a, b in _FP8_WIDE:
             n = -(-M // (32 * a)) * -(-N // (32 * b))
-            fill = 256 // n
+            fill = 256 // max(n, 1)
             plans += [(2, a, b, s) for s in {1, 2, 3, 4, fill // 2, fill}
                       if s == 1 or 1 < s <= min(fill + 1, 16) and s * 512 <= K]
     return min(plans, key=lambda p: (_fp8_time(*p, M, N, K), p))

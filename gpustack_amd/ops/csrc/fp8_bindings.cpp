@@ -185,18 +185,19 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
   const long T = order.size(0);
   TORCH_CHECK(starts.size(0) == S + 1 && ranks.size(0) == S,
               "lora_add: S + 1 starts and S ranks");
-  TORCH_CHECK(T <= rows && rows < 1l << 31 && S < 1l << 24 && N < 1l << 31 && K < 1l << 31,
-              "lora_add: sizes");
+  // the last: tiles of lists that name a row for every slot are still counted in 32 bits
+  TORCH_CHECK(T <= rows && rows < 1l << 31 && S < 1l << 24 && N < 1l << 31 &&
+              K < 1l << 31 && S * (T / 16 + 1) < 1l << 31, "lora_add: sizes");
   if (T == 0 || S == 0) return;
   const at::DeviceGuard guard(x.device());
-  // Tiles of 16 rows up to 767 rows in all, and below 32 a slot, else of 64, from 3072
+  // Tiles of 16 rows up to 767 rows in all, and below 32 a slot, else of 64, from 3000
   // rows and 192 a slot of 128. us in 16, 64 and 128: 128 rows of one slot, 6144 x 4096,
   // rank 16, 9.8, 13.7 and 15.6; 32 of each of 16 slots 16.2, 16.1 and 18.1, 64 of each
   // 21.5, 18.7 and 20.6; 256 of each of 4 slots, 28672 x 4096, 39.6, 35.9 and 37.1; of
   // each of 16, 4096 x 4096, rank 64, 66, 38.2 and 36.5
   const long used = std::min(S, T), groups = P * ((R + 15) / 16);
-  const LoraPlan plan = lora_plan(T < std::max(768l, 32 * used),
-                                  T >= std::max(3072l, 192 * used), (int)groups);
+  LoraPlan plan = lora_plan(T < std::max(768l, 32 * used),
+                                  T >= std::max(3000l, 192 * used), (int)groups);
   // k is cut until the workgroups fill the CUs: of few rows each wave has four units of
   // 64 k then; of many at least four steps are left, and up to five parts where the second
   // launch adds them up, 16 where one of their own does. One workgroup a CU: what a second
@@ -215,12 +216,19 @@ void lora_add(Tensor out, Tensor x, Tensor a, Tensor b, Tensor order, Tensor sta
   // 340 -> 306 us, 1200 of 6144 x 4096 at 128 38.6 -> 36.5; up to rank 32 2039 rows of
   // 6144 x 4096 26.1 -> 27.6)
   const bool join = !few && R > 32 && splits > 1;
-  // 256 columns of 16 to 64 rows at a time, more in turn where enough workgroups are left
-  const long up = lora_tiles(T, S, few ? 16 : R > 32 ? 64 : 32), across = (N + 255) / 256;
+  // The second launch: 256 columns of 32 rows at a time (of few, 16), more in turn where
+  // enough workgroups are left. 64 rows where each tile's way through b costs more than
+  // the registers that 64 take from other workgroups: above rank 128, and above 64 where
+  // neither a slot's b is short nor all of them stay in the L2s (us of 64 and of 32 rows:
+  // 8192 rows of 4096 columns at rank 64 71 and 61, 1852 of one slot, 15424 at 88 64 and
+  // 54, 1670 of 28, 2024 at 96 27.7 and 25.1; but 1933 of 11, 14296 at 112 58 and 80)
+  const long each = (long)N * R * 2;
+  const bool tall = !few && (R > 128 || (R > 64 && each > 1l << 20 && used * each > 6l << 20));
+  plan.up = few ? 1 : tall ? 4 : 2;
+  const long up = lora_tiles(T, S, 16 * plan.up), across = (N + 255) / 256;
   TORCH_CHECK(up <= 65535, "lora_add: sizes");
   const long turns = std::max(1l, few ? std::min(4l, up * across / 1024)
-                              : R > 32 ? std::min(4l, up * across / 512)
-                                       : std::min(2l, up * across / 512));
+                                      : std::min(tall ? 4l : 2l, up * across / 512));
   Tensor h = at::empty({splits, T, P * R}, x.options().dtype(at::kFloat)), joined;
   if (join) joined = at::empty({2, T, P * R}, x.options());
   lora_launch(out.data_ptr(), os, h.data_ptr<float>(), x.data_ptr(), xs, a.data_ptr(),

@@ -343,7 +343,8 @@ void fp8_wide_launch(void* out, const void* x, const float* xs, const void* w,
   *err_unsupported = K % 16 != 0 || K < FW_K || N % 8 != 0 ||
                      ((long)N + MOST) * K >= far || (long)K * MOST >= far ||
                      4l * N * (MOST + 1) >= (1l << 32) - 256 || splits < 1 ||
-                     ((K + FW_K - 1) / FW_K + 1) / 2 < splits || rf < 0 || rf > 9 || cf < 0 || cf > 9;
+                     ((K + FW_K - 1) / FW_K + 1) / 2 < splits || rf < 0 || rf > 9 ||
+                     cf < 0 || cf > 9;
   if (*err_unsupported || M == 0 || N == 0) return;
   switch ((splits > 1) * 100 + rf * 10 + cf) {
 #define WIDE(PARTS, RF, CF)                                                            \

@@ -4,8 +4,8 @@
 #include "common.h"
 
 // mt, nt: a tile of the first launch in 16 rows and columns; held: of its workgroups a CU
-// holds.
-struct LoraPlan { int mt, nt, held; };
+// holds; up: rows of the second in 16.
+struct LoraPlan { int mt, nt, held, up; };
 
 // Tiles of `each` rows that T rows of S slots can need: at most T slots have rows.
 static inline int lora_tiles(long T, long S, long each) {

@@ -11,11 +11,11 @@
 // higher ranks by a launch between the two), which holds them as two bf16 parts (the
 // value and what that rounded away, 16 bits of it in all): one would cost h the 2^-9 that
 // the rest of the sum does not lose. Both are bound by memory: x and a, then b and out.
-// us, first and second: one row of 4096 k and 6144 columns in three parts, rank 16, 4.2
-// and 4.5; 64 rows of 28 adapters, 28672 columns in two parts, ranks 1 to 64 of 64, 9 and
-// 27 (of rank 16 in 16, 6 and 9); 2039 rows of 8 runs, 6144 columns, rank 32, 12 and 14;
-// 8192 rows, 4096 columns, rank 64, 25 and 42 with 4 between, rank 16, 22 and 33; 28672
-// columns, rank 16, 24 and 207, where adding a number to as many takes 158.
+// us, first and second: one row of 4096 k and 6144 columns in three parts, rank 16, 4.1
+// and 4.6; 64 rows of 28 adapters, 28672 columns in two parts, ranks 1 to 64 of 64, 9 and
+// 27 (of rank 16 in 16, 6 and 10); 2039 rows of 8 runs, 6144 columns, rank 32, 12 and 15;
+// 8192 rows, 4096 columns, rank 64, 22 and 45 with 4 between, rank 16, 20 and 34; 28672
+// columns, rank 16, 22 and 203, where adding a number to as many takes 158.
 #include "lora.h"
 
 namespace {
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(
 // The same of prompts: tiles of 16 MT rows, and 16 NT of an adapter's columns, a step of
 // 64 k of both through a ring of S buffers in the LDS, filled S - 1 steps ahead (to the
 // registers, a wave with rows and columns of its own k, 8192 rows of 4096 k at 64 columns
-// take 33 us where these take DOWN_US). Rows of 128 bytes, 16-byte piece c of row r at
+// take 33 us where these take 23). Rows of 128 bytes, 16-byte piece c of row r at
 // c ^ (r / 2 % 8), which 16 rows read without conflict. Each of the four waves has MT / 4
 // tiles of rows and all columns, so there is nothing to add up in the workgroup.
 __device__ const u32x4 lora_zeros = {0, 0, 0, 0};
@@ -429,13 +429,14 @@ int lora_most_rank() { return 256; }
 // The tile's rows and columns of the first launch in 16, workgroups of it a CU holds.
 // few: 16 rows, one tile of columns; else by the tiles of columns that there are.
 LoraPlan lora_plan(bool few, bool many, int groups) {
-  if (few) return {1, 1, 8};
+  if (few) return {1, 1, 8, 1};
   const int nt = groups <= 2 ? 2 : groups <= 4 ? 4 : groups <= 8 ? 8 : 12;
-  return {many ? 8 : 4, nt, nt <= 4 ? 2 : 1};
+  return {many ? 8 : 4, nt, nt <= 4 ? 2 : 1, 2};
 }
 
 // rows: of x and out; T: entries of the order. K, R and the ends are multiples of 8.
-// splits: parts of k of h; parts: a place for its sums [2, T, P R], or null; turns: of 256 columns a workgroup of the second launch.
+// splits: parts of k of h; parts: a place for its sums [2, T, P R], or null; turns: of 256
+// columns a workgroup of the second launch.
 void lora_launch(void* out, long os, float* h, const void* x, long xs, const void* a,
                  const void* b, const int* order, const int* starts, const int* ranks,
                  int rows, int T, int S, int N, int K, int P, const int* ends, int R,
@@ -477,18 +478,17 @@ void lora_launch(void* out, long os, float* h, const void* x, long xs, const voi
                        (const unsigned short*)b, order, starts, ranks, rows, T, S, N, R,
                        turns, parts != nullptr, e);
   };
-  // Of many rows 32 a workgroup, which leave the registers room for more waves (28672
-  // columns at rank 16: 240 us, of 64 rows 307), but 64 where b is as long as what is
-  // read of out (rank 64: 243, of 32 rows 283).
-  if (plan.mt == 1) {
+  if (plan.up == 1) {
     if (R <= 32) up(lora_up_kernel<1, 1>, 1);
     else if (R <= 64) up(lora_up_kernel<1, 2>, 1);
     else if (R <= 128) up(lora_up_kernel<1, 4>, 1);
     else up(lora_up_kernel<1, 8>, 1);
-  } else {
+  } else if (plan.up == 2) {
     if (R <= 32) up(lora_up_kernel<2, 1>, 2);
-    else if (R <= 64) up(lora_up_kernel<4, 2>, 4);
-    else if (R <= 128) up(lora_up_kernel<4, 4>, 4);
+    else if (R <= 64) up(lora_up_kernel<2, 2>, 2);
+    else up(lora_up_kernel<2, 4>, 2);
+  } else {
+    if (R <= 128) up(lora_up_kernel<4, 4>, 4);
     else up(lora_up_kernel<4, 8>, 4);
   }
 }

@@ -77,6 +77,7 @@ def test_product_plans_are_the_kernels():
             # 32 bits of an operand's offsets and of a tile of the result's
             assert (N + 256) * K < 2 ** (31 if K % 128 else 32)
             assert 4 * N * 257 < 2 ** 32 - 256
+    ops._fp8_plan(70, 0, 128)        # a size that is refused behind it
 
 
 def test_batch_lists():

@@ -223,7 +223,8 @@ ADAPTERS = [  # rows, K, ends, slots, R, kind of batch
     (900, 72, (64, 200, 264), 4, 64, "prompts"), (800, 200, (88,), 3, 128, "prompts"),
     (1200, 40, (136, 328), 2, 256, "prompts"), (3300, 168, (72, 144), 2, 24, "prompts"),
     (3500, 128, (64,), 3, 64, "prompts"), (3100, 96, (32, 64, 96), 1, 48, "prompts"),
-    (3200, 64, (40, 80, 120, 160), 2, 72, "prompts"), (780, 264, (56,), 300, 16, "steps")]
+    (3200, 64, (40, 80, 120, 160), 2, 72, "prompts"), (780, 264, (56,), 300, 16, "steps"),
+    (800, 64, (8192,), 6, 72, "prompts"), (900, 64, (7000, 14336), 2, 48, "prompts")]
 
 
 def _slots(T, S, kind, seed):
