@@ -1191,8 +1191,9 @@ def convert_to_fp8_runtime(model, cfg: EngineConfig) -> int:
     (ops.add_rms_norm_fp8, silu_and_mul_fp8, rows_fp8; ops.linear_fp8). The
     embedding and the head keep their type, as do expert banks, latent
     attention and widths that the products do not take (N % 8, K % 16).
-    Returns the number of converted tensors. Reference capability: vLLM
-    --quantization fp8 with dynamic activation scales.
+    Returns the number of converted tensors; a model without any is refused.
+    Reference capability: vLLM --quantization fp8 with dynamic activation
+    scales.
     """
     from .. import ops
     from .llama import Attention, F8Pack, MLP
@@ -1203,9 +1204,10 @@ def convert_to_fp8_runtime(model, cfg: EngineConfig) -> int:
     n = 0
     for layer in model.layers:
         for mod, kind, sites in (
-                (layer.attn, Attention, (("qkv_w", "qkv_pack"), ("o_w", "o_pack"))),
-                (layer.mlp, MLP, (("gate_up_w", "gate_up_pack"),
-                                  ("down_w", "down_pack")))):
+                (getattr(layer, "attn", None), Attention,
+                 (("qkv_w", "qkv_pack"), ("o_w", "o_pack"))),
+                (getattr(layer, "mlp", None), MLP,
+                 (("gate_up_w", "gate_up_pack"), ("down_w", "down_pack")))):
             if not isinstance(mod, kind):
                 continue
             for wname, pname in sites:
@@ -1217,6 +1219,9 @@ def convert_to_fp8_runtime(model, cfg: EngineConfig) -> int:
                 setattr(mod, pname, F8Pack(r.q, r.scale, w.dtype))
                 w.data = torch.empty(0, dtype=w.dtype, device=w.device)
                 n += 1
+    if n == 0:
+        raise ValueError("quantize_runtime fp8: no projection of this model "
+                         "can be held in 8 bits")
     if model.device.type == "cuda":
         torch.cuda.empty_cache()
     return n

@@ -79,6 +79,17 @@ def test_one_layer_is_the_products_of_its_rounded_operands():
                           product(x, packs[0].qkv_pack).float(), rtol=2 ** -7, atol=1e-4)
 
 
+def test_models_without_a_projection_are_refused():
+    from types import SimpleNamespace
+
+    from gpustack_amd.models.weights import convert_to_fp8_runtime
+
+    model = SimpleNamespace(layers=[SimpleNamespace(mixer=None)],
+                            device=torch.device("cpu"))
+    with pytest.raises(ValueError, match="no projection"):
+        convert_to_fp8_runtime(model, EngineConfig(model="tiny", device="cpu"))
+
+
 def test_near_the_unconverted_engine():
     """Hidden states of 8-bit layers stay near: an e4m3 product's terms are off
     by up to 2^-4 on both sides, at random, so a sum of them by far less than
